@@ -160,6 +160,9 @@ int vox_hip_adapter_append(vox_hip_engine_t *e, const float *rows, int n_rows);
 int64_t vox_hip_adapter_rows(const vox_hip_engine_t *e);
 /* Device pointer of the adapter ring (for RCCL/torch interop) and its row capacity. */
 void *vox_hip_adapter_devptr(vox_hip_engine_t *e, int64_t *cap_rows);
+/* Device pointers of a decoder layer's K and V rings, [cap_rows, dec_kv_heads, dec_head_dim] f32, position p in row p % cap_rows (the
+ * caches of the operators in vox_hip_ops.h; reference: kv_cache_k / kv_cache_v, voxtral.h:154-204). */
+int vox_hip_decoder_kv_devptr(vox_hip_engine_t *e, int layer, void **k, void **v, int *cap_rows);
 
 /* ---- multi-GPU encoder sharding (exact context parallelism) ------
  * A rank owns encoder positions [pos0, pos0+n). Per layer it imports the layer's K/V of the

@@ -40,6 +40,7 @@
 using namespace vox;
 
 static thread_local std::string g_err;
+__attribute__((visibility("hidden"))) void vox_set_last_error(const char *text) { g_err = text; }      // (vox_ops.hip)
 static void set_err(const char *what, hipError_t e, const char *file, int line) {
     char buf[512];
     snprintf(buf, sizeof buf, "vox_hip: %s failed: %s (%s:%d)", what, hipGetErrorString(e), file, line);
@@ -1866,6 +1867,12 @@ extern "C" void *vox_hip_adapter_devptr(vox_hip_engine_t *e, int64_t *cap_rows) 
     if (!e) return nullptr;
     if (cap_rows) *cap_rows = e->adapter_cap;
     return e->adapter;
+}
+extern "C" int vox_hip_decoder_kv_devptr(vox_hip_engine_t *e, int layer, void **k, void **v, int *cap_rows) {
+    if (!e || !k || !v || !cap_rows) return -1;
+    if (layer < 0 || layer >= (int)e->dec.size()) { g_err = "vox_hip_decoder_kv_devptr: no such layer"; return -1; }
+    *k = e->dec[layer].kring; *v = e->dec[layer].vring; *cap_rows = e->dec_ring_cap;
+    return 0;
 }
 extern "C" int vox_hip_adapter_read(vox_hip_engine_t *e, int64_t first_row, int n_rows, float *out) {
     if (!e || n_rows <= 0) return -1;
