@@ -139,10 +139,52 @@ int check_attn(const vox_hip_tree_attn_t *a) {
     CHECK(a->reserved == 0, "%s: reserved is not 0", who);
     return 0;
 }
+
+// The matrix-pipe kernel takes 16-byte loads: every row of every operand starts on 16 bytes and holds whole loads, and rows of a cache
+// lie less than 2^31 bytes apart.  Everything else runs on the scalar kernel.
+bool attn_wide(const vox_hip_tree_attn_t *a) {
+    const int size = dtype_size(a->dtype), unit = 16 / size;
+    const void *p[5] = {a->q, a->k, a->v, a->k_cache, a->v_cache};
+    for (const void *x : p)
+        if (!aligned(x, 16)) return false;
+    const int64_t *st = &a->q_sb;
+    for (int i = 0; i < 15; i++)
+        if (st[i] % unit) return false;
+    const int64_t rows[4] = {a->k_st, a->v_st, a->kc_ss, a->vc_ss};
+    for (int64_t r : rows)
+        if (r * size >= (int64_t)1 << 31) return false;
+    return a->head_dim % unit == 0;
+}
+// Rows (nodes x heads of a kv head) per workgroup: all of them up to 128, so that keys are read once; a wave holds 16 or 32, as many as its
+// registers do.  Splits: enough workgroups for two per CU, but at least one key tile per wave in each.
+struct AttnLaunch { bool wide; int DP, RT, row_waves, row_blocks, splits; int64_t ws; unsigned lds; };
+AttnLaunch attn_launch(const vox_hip_tree_attn_t *a) {
+    AttnLaunch l{};
+    l.wide = attn_wide(a);
+    if (!l.wide || a->batch == 0 || a->nodes == 0) return l;
+    const int64_t R = (int64_t)a->nodes * (a->heads / a->kv_heads);
+    l.DP = a->head_dim <= 64 ? 64 : a->head_dim <= 128 ? 128 : 256;
+    l.RT = R <= 16 || l.DP == 256 ? 1 : 2;
+    const int waves = (int)((R + l.RT * 16 - 1) / (l.RT * 16));
+    l.row_waves = waves <= 1 ? 1 : waves <= 2 ? 2 : 4;
+    const int rows = l.RT * 16 * l.row_waves, key_waves = ATTN_WAVES / l.row_waves;
+    l.row_blocks = (int)((R + rows - 1) / rows);
+    l.lds = (unsigned)(rows * (l.DP + 4) + 2 * key_waves * rows) * 4;
+    const int KT = a->dtype == VOX_F32 ? 16 : 32;
+    const int64_t keys = a->window > 0 ? std::min(a->cap, a->window) : a->cap, tiles = (keys + KT - 1) / KT + (a->nodes + KT - 1) / KT;
+    const int64_t groups = (int64_t)a->batch * a->kv_heads * l.row_blocks;
+    l.splits = (int)std::max<int64_t>(1, std::min<int64_t>({64, 512 / groups, (tiles + key_waves - 1) / key_waves}));
+    if (l.splits > 1) l.ws = round_up((int64_t)l.splits * a->batch * a->kv_heads * R * a->head_dim * 4, 256) + (int64_t)l.splits * a->batch * a->kv_heads * R * 8;
+    return l;
+}
+template <typename T, int DP> void launch_attn(const TreeAttnArgs &t, const TreeAttnPlan &p, const AttnLaunch &l, dim3 grid, hipStream_t s) {
+    if (l.RT == 1) hipLaunchKernelGGL((k_tree_attn<T, DP, 1>), grid, dim3(64 * ATTN_WAVES), l.lds, s, t, p);
+    else if constexpr (DP < 256) hipLaunchKernelGGL((k_tree_attn<T, DP, 2>), grid, dim3(64 * ATTN_WAVES), l.lds, s, t, p);
+}
 }  // namespace
 extern "C" int64_t vox_hip_tree_attention_workspace(const vox_hip_tree_attn_t *a) {
     if (check_attn(a)) return -1;
-    return 0;
+    return attn_launch(a).ws;
 }
 extern "C" int vox_hip_tree_attention(const vox_hip_tree_attn_t *a, void *ws, size_t ws_bytes, int device, void *stream) {
     if (check_attn(a)) return -1;
@@ -150,14 +192,29 @@ extern "C" int vox_hip_tree_attention(const vox_hip_tree_attn_t *a, void *ws, si
     CHECK(a->q && a->k && a->v && a->k_cache && a->v_cache && a->cache_len && a->ancestors && a->depth && a->out, "vox_hip_tree_attention: null pointer");
     const int64_t *st = &a->q_sb;
     for (int i = 0; i < 18; i++) CHECK(st[i] >= 0, "vox_hip_tree_attention: negative stride");
+    const AttnLaunch l = attn_launch(a);
+    CHECK(l.ws == 0 || (ws && aligned(ws, 256) && ws_bytes >= (size_t)l.ws), "vox_hip_tree_attention: needs %lld bytes of workspace, 256-byte aligned", (long long)l.ws);
     OnDevice on("vox_hip_tree_attention", device);
     if (!on.ok) return -1;
     TreeAttnArgs t{a->q, a->k, a->v, a->k_cache, a->v_cache, a->cache_len, a->ancestors, a->depth, a->out, a->lse,
                    a->q_sb, a->q_st, a->q_sh, a->k_sb, a->k_st, a->k_sh, a->v_sb, a->v_st, a->v_sh, a->kc_sb, a->kc_ss, a->kc_sh, a->vc_sb, a->vc_ss, a->vc_sh,
                    a->o_sb, a->o_st, a->o_sh, a->nodes, a->heads, a->kv_heads, a->heads / a->kv_heads, a->head_dim, a->cap, a->window, (a->nodes + 63) / 64, a->scale};
-    (void)ws; (void)ws_bytes;
+    const hipStream_t s = (hipStream_t)stream;
+    if (!l.wide) {
+        by_type(a->dtype, [&](auto z) {
+            hipLaunchKernelGGL(k_tree_attn_scalar<decltype(z)>, dim3(a->nodes * a->heads, a->batch), dim3(256), 0, s, t);
+        });
+        return launched("vox_hip_tree_attention");
+    }
+    const int R = a->nodes * t.G;
+    TreeAttnPlan p{l.splits, l.row_blocks, l.row_waves, (float *)ws, (float *)((char *)ws + round_up((int64_t)l.splits * a->batch * a->kv_heads * R * a->head_dim * 4, 256))};
+    const dim3 grid((unsigned)(round_up((int64_t)l.splits * a->kv_heads, 8) * l.row_blocks), a->batch);
     by_type(a->dtype, [&](auto z) {
-        hipLaunchKernelGGL(k_tree_attn_scalar<decltype(z)>, dim3(a->nodes * a->heads, a->batch), dim3(256), 0, (hipStream_t)stream, t);
+        typedef decltype(z) T;
+        if (l.DP == 64) launch_attn<T, 64>(t, p, l, grid, s);
+        else if (l.DP == 128) launch_attn<T, 128>(t, p, l, grid, s);
+        else launch_attn<T, 256>(t, p, l, grid, s);
+        if (l.splits > 1) hipLaunchKernelGGL(k_tree_attn_join<T>, dim3((R + 3) / 4, a->kv_heads, a->batch), dim3(256), 0, s, t, p);
     });
     return launched("vox_hip_tree_attention");
 }

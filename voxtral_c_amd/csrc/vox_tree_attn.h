@@ -85,4 +85,426 @@ template <typename T> __global__ __launch_bounds__(256) void k_tree_attn_scalar(
     if (a.lse && threadIdx.x == 0) a.lse[((size_t)b * a.T + i) * a.H + h] = mm + logf(total);
 }
 
+
+// ---- matrix-pipe form ----------------------------------------------------------------------------------------------------------
+// The G query heads of a kv head share its keys, so the rows of a (sequence, kv head) are its nodes x G heads, taken in tiles of 16.  A wave
+// owns KT keys at a time and both products are transposed so that nothing passes through LDS:
+//   S^T[key, row] = K . Q^T      K is the A operand (lane: key = lane % 16, its share of the head's dimensions), Q^T stays in registers;
+//   O^T[d, row]  += V^T . P^T    the lane that holds S^T's column (row = lane % 16) for keys 4 c + r, c = lane / 16, holds exactly
+//                                what the B operand wants of P^T if the product's inner index runs over keys in that order, and V is loaded as the
+//                                A operand in the same order: lane m of a 16-lane row takes E = DP / 16 consecutive dimensions of the keys 4 c + r
+//                                and supplies dimension m E + e to the e-th product.
+// Every key and value is loaded once per row block, straight from memory into the registers that the matrix instruction reads, 16 bytes per lane; K of
+// the next tile is requested when the scores are done, V when the outputs are.  Each wave runs its own online softmax (one maximum and sum per
+// row); the waves of a workgroup are joined through LDS at the end, the parts of a long cache by k_tree_attn_join.
+template <typename T> struct AttnType;
+template <> struct AttnType<float> {
+    static constexpr int KT = 16, SHIFT = 0;
+    typedef unsigned Bits;
+    static constexpr Bits INF = 0x7f800000u, SIGN = 0x80000000u;
+    static constexpr float LAZY = 8.f;
+};
+// P is rounded to bf16 in front of its product (a half step of 2^-8 per weight, like the rounding of the output itself): the product then runs at
+// the 16-bit rate.  The weights' sum is taken of the f32 values.
+template <> struct AttnType<bf16_t> {
+    static constexpr int KT = 32, SHIFT = 0;
+    typedef unsigned short Bits;
+    static constexpr Bits INF = 0x7f80, SIGN = 0x8000;
+    static constexpr float LAZY = 8.f;
+};
+// f16: the same with a half step of 2^-11; weights are lifted by 2^12 so that what is 2^-26 of the largest one is still a normal number (a sum over
+// tens of thousands of small weights would lose them otherwise).
+template <> struct AttnType<f16_t> {
+    static constexpr int KT = 32, SHIFT = 12;
+    typedef unsigned short Bits;
+    static constexpr Bits INF = 0x7c00, SIGN = 0x8000;
+    static constexpr float LAZY = 3.f;
+};
+
+constexpr int ATTN_WAVES = 4;
+// The waves of a workgroup: row_waves of them side by side over the rows (each RT row tiles, the same keys: they share them through L1), the
+// others (key_waves = ATTN_WAVES / row_waves) over the keys.
+struct TreeAttnPlan {
+    int splits, row_blocks, row_waves;
+    float *part_o, *part_ml;      // [splits][batch * Hk][rows][D], [splits][batch * Hk][rows][2]
+};
+
+__device__ __forceinline__ float max_over_c(float v) {        // over lanes l, l ^ 16, l ^ 32, l ^ 48
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum_over_c(float v) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// One step of 16 x 16 outputs: an inner index of 32 (16-bit types, 8 values per lane) or 16 (f32: four instructions of 4).
+template <typename T, typename V> __device__ __forceinline__ f32x4 attn_mma(const V x, const V y, f32x4 acc) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], acc, 0, 0, 0);
+        return acc;
+    } else if constexpr (__is_same(T, bf16_t)) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, acc, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, acc, 0, 0, 0);
+}
+
+// Key tiles of a sequence: the cache's, then the tree's; split s takes tiles [s * per, (s + 1) * per).
+struct TileRange {
+    int64_t first, len;
+    int cached, n_cache, n_all, per;
+};
+template <int KT> __device__ __forceinline__ TileRange tile_range(const TreeAttnArgs &a, int b, const TreeAttnPlan &plan) {
+    TileRange r;
+    tree_range(a, b, r.first, r.len);
+    r.cached = (int)(r.len - r.first);
+    r.n_cache = (int)(((int64_t)r.cached + KT - 1) / KT);
+    r.n_all = r.n_cache + (a.T + KT - 1) / KT;
+    const int kw = ATTN_WAVES / plan.row_waves;
+    r.per = ((r.n_all + plan.splits - 1) / plan.splits + kw - 1) / kw * kw;
+    return r;
+}
+
+// One tile's keys: row `base`, key i in row base + (i < wrap ? i : i - cap), `count` of them.
+struct KeyTile {
+    const char *k, *v;
+    int ks, vs;                   // bytes between rows
+    int count, wrap, cap;
+};
+
+template <typename T, int DP, int RT> __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_attn(TreeAttnArgs a, TreeAttnPlan plan) {
+    typedef AttnType<T> A;
+    constexpr int KT = A::KT, E = DP / 16, NK = KT / 16, VK = KT / 4;            // VK: keys per lane of a V operand
+    constexpr int U = sizeof(T) == 2 ? 8 : 4;                                    // elements per 16-byte load
+    constexpr int KS = DP / (4 * U);                                             // K / Q loads per lane and 16 keys / rows
+    constexpr int VU = E < U ? E : U, VL = E / VU;                               // V: VL loads of VU elements per key
+    constexpr float LOG2E = 1.44269504088896340736f;
+    typedef T kvec __attribute__((ext_vector_type(U)));
+    typedef T vvec __attribute__((ext_vector_type(VU)));
+    constexpr int WROWS = RT * 16, LD = DP + 4;                                  // rows of a wave
+    const int RW = plan.row_waves, KW = ATTN_WAVES / RW, ROWS = WROWS * RW;      // rows of a workgroup
+    extern __shared__ __attribute__((aligned(16))) float so[];                   // [ROWS][LD]: Q^T during the loop, then the outputs, one key wave's after another's
+    float *sm = so + ROWS * LD, *sl = sm + KW * ROWS;                            // [KW][ROWS] each
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kw = wave / RW, rw = wave - kw * RW, n16 = lane & 15, c = lane >> 4;
+    // Workgroups that read the same keys (the row blocks of a group) have numbers that differ by 8: they land on one XCD and share its L2.
+    const int RB = plan.row_blocks, chunk = blockIdx.x / (8 * RB), in = blockIdx.x - chunk * 8 * RB;
+    const int group = chunk * 8 + (in & 7), rb = in >> 3;
+    const int b = blockIdx.y, split = group / a.Hk, kvh = group - split * a.Hk;
+    if (split >= plan.splits) return;
+    const TileRange tr = tile_range<KT>(a, b, plan);
+    const int t_begin = split * tr.per, t_end = min(t_begin + tr.per, tr.n_all);
+    if (t_begin >= t_end) return;
+    const int R = a.T * a.G, row0 = rb * ROWS, wrow0 = row0 + rw * WROWS;
+    const bool idle = wrow0 >= R;                            // (the last workgroup's waves behind the last row)
+
+    // this lane's query rows
+    int row_depth[RT], row_node[RT];
+    // Q^T as B operands: in registers, or in LDS [RT][KS][64 lanes] where the registers do not hold them (f32, 256 dimensions)
+    constexpr bool QLDS = sizeof(T) == 4 || DP == 256;
+    kvec qf[QLDS ? 1 : RT][QLDS ? 1 : KS];
+    kvec *qs = reinterpret_cast<kvec *>(so) + rw * RT * KS * 64;
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const int row = wrow0 + t * 16 + n16, node = row < R ? row / a.G : 0, h = kvh * a.G + (row - node * a.G);
+        row_node[t] = node;
+        row_depth[t] = row < R ? a.depth[(size_t)b * a.T + node] : -1;
+        const T *q = (const T *)a.q + b * a.q_sb + node * a.q_st + h * a.q_sh;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            const int d = s * 4 * U + c * U;
+            kvec x = kvec(T(0.f));
+            if (row < R && d < a.D) x = *reinterpret_cast<const kvec *>(q + d);
+            if constexpr (!QLDS) qf[t][s] = x;
+            else if (kw == 0) qs[(t * KS + s) * 64 + lane] = x;
+        }
+    }
+    if (QLDS) __syncthreads();
+    const char *kc = (const char *)((const T *)a.kc + b * a.kc_sb + kvh * a.kc_sh), *vc = (const char *)((const T *)a.vc + b * a.vc_sb + kvh * a.vc_sh);
+    const char *kt = (const char *)((const T *)a.k + b * a.k_sb + kvh * a.k_sh), *vt = (const char *)((const T *)a.v + b * a.v_sb + kvh * a.v_sh);
+    const int64_t slot_first = tr.first % a.cap;
+    auto tile_at = [&](int t) {
+        KeyTile x;
+        if (t < tr.n_cache) {
+            const int off = t * KT;
+            int64_t slot = slot_first + off;
+            if (slot >= a.cap) slot -= a.cap;
+            x.k = kc + slot * a.kc_ss * (int)sizeof(T);
+            x.v = vc + slot * a.vc_ss * (int)sizeof(T);
+            x.ks = (int)(a.kc_ss * (int)sizeof(T));
+            x.vs = (int)(a.vc_ss * (int)sizeof(T));
+            x.count = min(KT, tr.cached - off);
+            x.wrap = (int)min((int64_t)KT, a.cap - slot);
+        } else {
+            const int off = (t - tr.n_cache) * KT;
+            x.k = kt + off * a.k_st * (int)sizeof(T);
+            x.v = vt + off * a.v_st * (int)sizeof(T);
+            x.ks = (int)(a.k_st * (int)sizeof(T));
+            x.vs = (int)(a.v_st * (int)sizeof(T));
+            x.count = min(KT, a.T - off);
+            x.wrap = KT;
+        }
+        x.cap = a.cap;
+        return x;
+    };
+    // Does every row see the whole tile?  And which of its keys (bit i) does row tile r's row of this lane see?
+    auto is_masked = [&](int t, const KeyTile &x) {
+        return t >= tr.n_cache || x.count < KT || (a.window > 0 && tr.first + (int64_t)t * KT <= tr.len + a.T - a.window);
+    };
+    auto visible = [&](int t, const KeyTile &x, int r) {
+        unsigned bits = 0xffffffffu;
+        if (t >= tr.n_cache) {
+            const int off = (t - tr.n_cache) * KT;
+            bits = (unsigned)(a.ancestors[((size_t)b * a.T + row_node[r]) * a.W + (off >> 6)] >> (off & 63));
+            if (a.window > 0)
+                for (int j = 0; j < x.count; j++)
+                    if (a.depth[(size_t)b * a.T + off + j] <= row_depth[r] - a.window) bits &= ~(1u << j);
+        } else if (a.window > 0) {
+            const int64_t below = tr.len + row_depth[r] - a.window - (tr.first + (int64_t)t * KT) + 1;       // keys in front of the row's window
+            bits = below >= 32 ? 0u : below <= 0 ? 0xffffffffu : 0xffffffffu << (int)below;
+        }
+        return x.count < 32 ? bits & ((1u << x.count) - 1u) : bits;
+    };
+    kvec kf[NK][KS];
+    vvec vf[VK][VL];
+    auto load_k = [&](const KeyTile &x) {
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+            const int key = i * 16 + n16, row = key < x.wrap ? key : key - x.cap;
+            const T *p = reinterpret_cast<const T *>(x.k + (int64_t)row * x.ks);
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                const int d = s * 4 * U + c * U;
+                if (key < x.count && d < a.D) kf[i][s] = *reinterpret_cast<const kvec *>(p + d);
+                else kf[i][s] = kvec(T(0.f));
+            }
+        }
+    };
+    auto load_v = [&](const KeyTile &x) {
+#pragma unroll
+        for (int j = 0; j < VK; j++) {
+            const int key = (j >> 2) * 16 + c * 4 + (j & 3), row = key < x.wrap ? key : key - x.cap;
+            const T *p = reinterpret_cast<const T *>(x.v + (int64_t)row * x.vs);
+#pragma unroll
+            for (int u = 0; u < VL; u++) {
+                const int d = n16 * E + u * VU;
+                if (key < x.count && d < a.D) vf[j][u] = *reinterpret_cast<const vvec *>(p + d);
+                else vf[j][u] = vvec(T(0.f));
+            }
+        }
+    };
+
+    f32x4 o[RT][E];
+    float m[RT], l[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        m[t] = -INFINITY; l[t] = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; e++) o[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const float scale2 = a.scale * LOG2E;
+    typedef typename A::Bits bits_t;
+    auto bits_of = [](T x) { return __builtin_bit_cast(bits_t, x); };
+    bool bad = false;                                        // a masked tile of this wave held a value that is not finite
+
+    int t = idle ? t_end : t_begin + kw;
+    KeyTile cur{}, nxt{};
+    if (t < t_end) { cur = tile_at(t); load_k(cur); load_v(cur); }
+    for (; t < t_end; t += KW, cur = nxt) {
+        const bool more = t + KW < t_end;
+        if (more) nxt = tile_at(t + KW);
+        const bool masked = is_masked(t, cur);
+        kvec pf[RT];                                         // the row tiles' weights as the second product's operand
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            f32x4 s[NK];
+#pragma unroll
+            for (int i = 0; i < NK; i++) {
+                s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int x = 0; x < KS; x++) {
+                    kvec q;
+                    if constexpr (QLDS) q = qs[(r * KS + x) * 64 + lane];
+                    else q = qf[r][x];
+                    s[i] = attn_mma<T>(kf[i][x], q, s[i]);
+                }
+                s[i] *= scale2;
+            }
+            if (masked) {
+                const unsigned bits = visible(t, cur, r);
+#pragma unroll
+                for (int i = 0; i < NK; i++)
+#pragma unroll
+                    for (int y = 0; y < 4; y++)
+                        if (!((bits >> (i * 16 + c * 4 + y)) & 1u)) s[i][y] = -INFINITY;
+            }
+            // online softmax, base 2; the maximum is only raised when it grows by more than LAZY (weights stay below 2^(LAZY + SHIFT))
+            float mx = s[0][0];
+#pragma unroll
+            for (int i = 0; i < NK; i++)
+#pragma unroll
+                for (int y = 0; y < 4; y++) mx = fmaxf(mx, s[i][y]);
+            mx = max_over_c(mx);
+            if (__any(mx > m[r] + A::LAZY)) {
+                const float mn = fmaxf(m[r], mx), f = mn == m[r] ? 1.f : __builtin_amdgcn_exp2f(m[r] - mn);
+                l[r] *= f;
+                m[r] = mn;
+#pragma unroll
+                for (int e = 0; e < E; e++) o[r][e] *= f;
+            }
+            const float base = (m[r] == -INFINITY ? 0.f : m[r]) - A::SHIFT;
+#pragma unroll
+            for (int i = 0; i < NK; i++)
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    s[i][y] = __builtin_amdgcn_exp2f(s[i][y] - base);
+                    l[r] += s[i][y];
+                    pf[r][i * 4 + y] = from_f32<T>(s[i][y]);
+                }
+        }
+        if (more) load_k(nxt);
+        auto v_operand = [&](int e) {
+            kvec av;
+#pragma unroll
+            for (int j = 0; j < VK; j++) av[j] = vf[j][e / VU][e % VU];
+            return av;
+        };
+        if (masked) {
+            // 0 * inf: a value that is not finite must not reach the rows that do not see its key.  It becomes zero here; what it does to the rows
+            // that see it is put in behind the loop.
+#pragma unroll
+            for (int j = 0; j < VK; j++)
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if ((bits_of(vf[j][e / VU][e % VU]) & A::INF) == A::INF) { vf[j][e / VU][e % VU] = T(0.f); bad = true; }
+        }
+        // O^T += V^T P^T
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const kvec av = v_operand(e);
+#pragma unroll
+            for (int r = 0; r < RT; r++) o[r][e] = attn_mma<T>(av, pf[r], o[r][e]);
+        }
+        if (more) load_v(nxt);
+    }
+    if (__any(bad)) {
+        // Per masked tile and kind (+inf, -inf, NaN): how many such values a row sees is a product of ones; one makes the sum that kind.
+        for (t = t_begin + kw; t < t_end; t += KW) {
+            cur = tile_at(t);
+            if (!is_masked(t, cur)) continue;
+            load_v(cur);
+#pragma unroll 1
+            for (int kind = 0; kind < 3; kind++) {
+                const float value = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN;
+                const bits_t inf = kind == 0 ? A::INF : (bits_t)(A::INF | A::SIGN);
+#pragma unroll
+                for (int r = 0; r < RT; r++) {
+                    const unsigned sees = visible(t, cur, r);
+                    kvec one;
+#pragma unroll
+                    for (int j = 0; j < VK; j++) one[j] = (sees >> ((j >> 2) * 16 + c * 4 + (j & 3))) & 1u ? T(1.f) : T(0.f);
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        kvec is;
+#pragma unroll
+                        for (int j = 0; j < VK; j++) {
+                            const bits_t x = bits_of(vf[j][e / VU][e % VU]);
+                            is[j] = (kind == 2 ? (bits_t)(x & ~A::SIGN) > A::INF : x == inf) ? T(1.f) : T(0.f);
+                        }
+                        const f32x4 n = attn_mma<T>(is, one, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                        for (int y = 0; y < 4; y++)
+                            if (n[y] > 0.f) o[r][e][y] += value;
+                    }
+                }
+            }
+        }
+    }
+    __syncthreads();
+
+    // join the key waves: common maximum, then the outputs one wave after another (a fixed order)
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+        l[r] = sum_over_c(l[r]);
+        if (c == 0) { sm[kw * ROWS + rw * WROWS + r * 16 + n16] = m[r]; sl[kw * ROWS + rw * WROWS + r * 16 + n16] = l[r]; }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+        const int row = rw * WROWS + r * 16 + n16;
+        float mm = sm[row];
+        for (int w = 1; w < KW; w++) mm = fmaxf(mm, sm[w * ROWS + row]);
+        const float f = m[r] == mm ? 1.f : __builtin_amdgcn_exp2f(m[r] - mm);
+#pragma unroll
+        for (int e = 0; e < E; e++) o[r][e] *= f;
+    }
+    for (int w = 0; w < KW; w++) {
+        if (w == kw) {
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+#pragma unroll
+                for (int y = 0; y < 4; y++)
+#pragma unroll
+                    for (int e = 0; e < E; e += 4) {
+                        f32x4 *dst = reinterpret_cast<f32x4 *>(&so[(rw * WROWS + r * 16 + n16) * LD + (c * 4 + y) * E + e]);
+                        const f32x4 x = {o[r][e][y], o[r][e + 1][y], o[r][e + 2][y], o[r][e + 3][y]};
+                        *dst = w == 0 ? x : *dst + x;
+                    }
+        }
+        __syncthreads();
+    }
+    const bool whole = tr.per >= tr.n_all;                   // one split holds all keys of this sequence
+    const int64_t prow = ((int64_t)split * gridDim.y + b) * a.Hk + kvh;
+    for (int row = wave; row < ROWS && row0 + row < R; row += ATTN_WAVES) {
+        float mm = sm[row], total = 0.f;
+        for (int w = 1; w < KW; w++) mm = fmaxf(mm, sm[w * ROWS + row]);
+        for (int w = 0; w < KW; w++) total += sl[w * ROWS + row] * (sm[w * ROWS + row] == mm ? 1.f : __builtin_amdgcn_exp2f(sm[w * ROWS + row] - mm));
+        const int grow = row0 + row, node = grow / a.G, h = kvh * a.G + (grow - node * a.G);
+        if (whole) {
+            const bool none = total == 0.f || a.depth[(size_t)b * a.T + node] < 0;
+            T *out = (T *)a.out + b * a.o_sb + node * a.o_st + h * a.o_sh;
+            for (int d = lane; d < a.D; d += 64) out[d] = from_f32<T>(none ? 0.f : so[row * LD + d] / total);
+            if (a.lse && lane == 0) a.lse[((size_t)b * a.T + node) * a.H + h] = none ? -INFINITY : (mm - A::SHIFT + log2f(total)) * 0.693147180559945309417f;
+        } else {
+            for (int d = lane; d < a.D; d += 64) plan.part_o[(prow * R + grow) * a.D + d] = so[row * LD + d];
+            if (lane == 0) { plan.part_ml[(prow * R + grow) * 2] = mm; plan.part_ml[(prow * R + grow) * 2 + 1] = total; }
+        }
+    }
+}
+
+// Joins the parts of a row: one wave per (row, kv head, sequence); grid (ceil(rows / 4), Hk, batch).
+template <typename T> __global__ __launch_bounds__(256) void k_tree_attn_join(TreeAttnArgs a, TreeAttnPlan plan) {
+    typedef AttnType<T> A;
+    const int lane = threadIdx.x & 63, R = a.T * a.G, row = blockIdx.x * 4 + (threadIdx.x >> 6), kvh = blockIdx.y, b = blockIdx.z;
+    if (row >= R) return;
+    const TileRange tr = tile_range<A::KT>(a, b, plan);
+    const int n = (tr.n_all + tr.per - 1) / tr.per;
+    if (n <= 1) return;                                      // written by its only part
+    const int64_t step = (int64_t)gridDim.z * a.Hk * R, at = ((int64_t)b * a.Hk + kvh) * R + row;
+    float mm = -INFINITY;
+    for (int s = lane; s < n; s += 64) mm = fmaxf(mm, plan.part_ml[(s * step + at) * 2]);
+    mm = wave_max(mm);
+    float total = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < n; s++) {
+        const float ms = plan.part_ml[(s * step + at) * 2], f = ms == mm ? 1.f : __builtin_amdgcn_exp2f(ms - mm);
+        total += f * plan.part_ml[(s * step + at) * 2 + 1];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int d = lane + 64 * j;
+            if (d < a.D) acc[j] += f * plan.part_o[(s * step + at) * a.D + d];
+        }
+    }
+    const int node = row / a.G, h = kvh * a.G + (row - node * a.G);
+    const bool none = total == 0.f || a.depth[(size_t)b * a.T + node] < 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int d = lane + 64 * j;
+        if (d < a.D) ((T *)a.out)[b * a.o_sb + node * a.o_st + h * a.o_sh + d] = from_f32<T>(none ? 0.f : acc[j] / total);
+    }
+    if (a.lse && lane == 0) a.lse[((size_t)b * a.T + node) * a.H + h] = none ? -INFINITY : (mm - A::SHIFT + log2f(total)) * 0.693147180559945309417f;
+}
+
 }  // namespace vox
