@@ -387,7 +387,8 @@ def check_linear(x, w, ws, bias, dtype):
 
 
 I8 = [(1, 64, 16), (1, 1280, 6144), (2, 100, 7), (3, 1, 5), (5, 128, 1000), (16, 256, 48), (17, 320, 130), (25, 5120, 1280), (33, 80, 64), (64, 4096, 33), (65, 1008, 257), (130, 192, 96),
-      (200, 1280, 520), (257, 2064, 129), (1000, 64, 65), (300, 77, 200), (128, 128, 128), (256, 512, 256), (513, 640, 768)]
+      (200, 1280, 520), (257, 2064, 129), (1000, 64, 65), (300, 77, 200), (128, 128, 128), (256, 512, 256), (513, 640, 768),
+      (700, 144, 5500), (1030, 208, 8000)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])

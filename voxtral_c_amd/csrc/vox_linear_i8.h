@@ -27,19 +27,33 @@ __device__ __forceinline__ RowScale row_scale(unsigned amax_bits) {
     return r;
 }
 
-// One workgroup per row: q [rows, ldq] (columns K .. ldq - 1 are zeros), scale [rows].  Bound by the row's two trips (the second one hits L2).
-template <typename T> __global__ __launch_bounds__(256) void k_quant_rows_i8(const T *x, int64_t stride, int K, int ldq, int8_t *q, float *scale) {
+// One workgroup per row: q [rows, ldq] (columns K .. ldq - 1 are zeros), scale [rows].  Bound by the row's two trips (the second one hits the
+// caches).  N elements per load: K, stride and x allow it, and ldq % N = 0.
+template <typename T, int N> __global__ __launch_bounds__(256) void k_quant_rows_i8(const T *x, int64_t stride, int K, int ldq, int8_t *q, float *scale) {
     __shared__ unsigned red[4];
     const int64_t row = blockIdx.x;
     const T *xr = x + row * stride;
     int8_t *qr = q + row * ldq;
     unsigned m = 0;
-    for (int k = threadIdx.x; k < K; k += 256) m = max(m, __float_as_uint((float)xr[k]) & 0x7fffffffu);
+    for (int k = threadIdx.x * N; k < K; k += 256 * N) {
+        float v[N];
+        load_vec<T, N>(v, xr + k);
+#pragma unroll
+        for (int i = 0; i < N; i++) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    }
     m = wave_max_u(m);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
     __syncthreads();
     const RowScale r = row_scale(max(max(red[0], red[1]), max(red[2], red[3])));
-    for (int k = threadIdx.x; k < ldq; k += 256) qr[k] = k < K && !r.broken ? (int8_t)quant_i8((float)xr[k], r.s, r.inv) : (int8_t)0;
+    for (int k = threadIdx.x * N; k < ldq; k += 256 * N) {
+        typedef int8_t out __attribute__((ext_vector_type(N)));
+        float v[N] = {};
+        out o;
+        if (k < K && !r.broken) load_vec<T, N>(v, xr + k);
+#pragma unroll
+        for (int i = 0; i < N; i++) o[i] = (int8_t)(int)quant_i8(v[i], r.s, r.inv);
+        *reinterpret_cast<out *>(qr + k) = o;
+    }
     if (threadIdx.x == 0) scale[row] = r.broken ? NAN : r.s;
 }
 
@@ -88,6 +102,154 @@ template <typename T> __global__ __launch_bounds__(256) void k_linear_i8_bytes(L
             const int m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
             if (m < a.M && n < a.N) ((T *)a.y)[m * a.y_stride + n] = i8_out<T>(acc[i][j], a.xs[m], a.ws[n], (const T *)a.bias, n);
         }
+}
+
+
+// ---- few rows: a read of the weights --------------------------------------------------------------------------------------------
+// A workgroup makes 16 output channels of MT x 16 rows; its waves split K and their whole-number sums are added through LDS (exact in any order).
+// v_mfma_i32_16x16x64_i8 with the weights as A operand: lane = (channel lane % 16, 16 bytes of K), loaded straight from the row-major matrix, 64 bytes of
+// each of 16 rows per instruction and two neighbouring instructions per 128-byte line.
+constexpr int I8_ROWS_WAVES = 8;
+template <typename T, int MT> __global__ __launch_bounds__(64 * I8_ROWS_WAVES) void k_linear_i8_rows(LinearI8Args a) {
+    __shared__ i32x4 part[I8_ROWS_WAVES][MT][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, c = lane >> 4;
+    const int n0 = blockIdx.x * 16;
+    const int8_t *w = a.w + (int64_t)min(n0 + n16, a.N - 1) * a.w_stride + c * 16;
+    const int8_t *x[MT];
+#pragma unroll
+    for (int t = 0; t < MT; t++) x[t] = a.xq + (int64_t)min(t * 16 + n16, a.M - 1) * a.ldq + c * 16;
+    i32x4 acc[MT] = {};
+    for (int k = wave * 128; k < a.K; k += 128 * I8_ROWS_WAVES) {
+        // (xq holds zeros from K to ldq, a multiple of 128: what stands in for weights behind K does not matter, so it is the row's first bytes)
+        const i32x4 w0 = *reinterpret_cast<const i32x4 *>(w + (k + c * 16 < a.K ? k : -c * 16));
+        const i32x4 w1 = *reinterpret_cast<const i32x4 *>(w + (k + 64 + c * 16 < a.K ? k + 64 : -c * 16));
+#pragma unroll
+        for (int t = 0; t < MT; t++) {
+            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w0, *reinterpret_cast<const i32x4 *>(x[t] + k), acc[t], 0, 0, 0);
+            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w1, *reinterpret_cast<const i32x4 *>(x[t] + k + 64), acc[t], 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; t++) part[wave][t][lane] = acc[t];
+    __syncthreads();
+    for (int i = tid; i < MT * 256; i += 64 * I8_ROWS_WAVES) {
+        // channel i % 16 of row i / 16: element (channel % 4) of lane (channel / 4) * 16 + row % 16
+        const int ch = i & 15, row = i >> 4, n = n0 + ch;
+        int sum = 0;
+#pragma unroll
+        for (int v = 0; v < I8_ROWS_WAVES; v++) sum += reinterpret_cast<const int *>(&part[v][row >> 4][(ch >> 2) * 16 + (row & 15)])[ch & 3];
+        if (row < a.M && n < a.N) ((T *)a.y)[row * a.y_stride + n] = i8_out<T>(sum, a.xs[row], a.ws[n], (const T *)a.bias, n);
+    }
+}
+
+// ---- many rows: a matrix product ------------------------------------------------------------------------------------------------
+// BM rows x 128 channels per workgroup of four waves (2 x 2, each BM / 2 rows x 64 channels) on v_mfma_i32_32x32x32_i8.  Slices of 128 bytes of K
+// go from memory into LDS without registers (global_load_lds_dwordx4: a wave's instruction brings 128 bytes of each of 8 rows), STAGES of them in
+// flight with one barrier per slice.  16-byte pieces of a row are stored at (piece ^ (row & 7)): the MFMA operand reads (lane = row, one piece) then
+// touch every bank once.  Outputs leave through LDS so that rows are written in whole lines.
+constexpr int I8_BN = 128, I8_BK = 128;
+template <typename T, int BM, int STAGES> __global__ __launch_bounds__(256) void k_linear_i8_tile(LinearI8Args a, int tiles_m, int tiles_n) {
+    typedef int i32x16 __attribute__((ext_vector_type(16)));
+    constexpr int ROWS = BM + I8_BN, STAGE = ROWS * I8_BK, LOADS = ROWS / 32;      // LOADS: instructions per wave and slice
+    constexpr int MI = BM / 64, NJ = 2;                                            // 32 x 32 blocks of a wave: rows, channels
+    extern __shared__ __attribute__((aligned(128))) int8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
+    // Each XCD (workgroup number mod 8) works through a range of tiles of its own in which the channels change fastest within bands of an
+    // eighth of all channels: its L2 keeps the band's weights, and a row panel is read once per band.
+    const int total = tiles_m * tiles_n, per = (total + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || id >= total) return;
+    const int band_n = (tiles_n + 7) / 8, band = id / (tiles_m * band_n), in = id - band * tiles_m * band_n;
+    const int width = min(band_n, tiles_n - band * band_n), tm = in / width, tn = band * band_n + in - tm * width;
+    const int m0 = tm * BM, n0 = tn * I8_BN;
+
+    // this lane's pieces: rows of x first, then rows of w; pieces behind K are the row's first one (x holds zeros there)
+    const int piece = lane & 7;
+    const int8_t *src[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) {
+        const int row = (i * 4 + wave) * 8 + (lane >> 3), p = piece ^ (row & 7);
+        src[i] = i * 32 >= BM ? a.w + (int64_t)min(n0 + row - BM, a.N - 1) * a.w_stride + p * 16 : a.xq + (int64_t)min(m0 + row, a.M - 1) * a.ldq + p * 16;
+    }
+    const int slices = a.ldq / I8_BK;
+    auto issue = [&](int s) {
+        const unsigned base = lds_addr(lds) + (s % STAGES) * STAGE;
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int row = (i * 4 + wave) * 8 + (lane >> 3), p = (piece ^ (row & 7)) * 16;
+            const bool past = i * 32 >= BM && s * I8_BK + p >= a.K;
+            glds16(src[i] + (past ? -p : s * I8_BK), __builtin_amdgcn_readfirstlane(base + (i * 4 + wave) * 1024));
+        }
+    };
+    i32x16 acc[NJ][MI] = {};
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; s++)
+        if (s < slices) issue(s);
+    for (int s = 0; s < slices; s++) {
+        // slice s has landed when at most the younger slices' loads are in flight; behind the barrier everyone's has, and everyone is done with the
+        // slice that the next loads overwrite
+        // (this wave's own LDS reads of that slice have returned too: the compiler may place the products that use them behind the barrier)
+        if (STAGES == 3 && s + 1 < slices) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (s + STAGES - 1 < slices) issue(s + STAGES - 1);
+        const int8_t *buf = lds + (s % STAGES) * STAGE;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            i32x4 wf[NJ], xf[MI];
+            const int q = k * 2 + (lane >> 5);
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                const int row = BM + wn * 64 + j * 32 + (lane & 31);
+                wf[j] = *reinterpret_cast<const i32x4 *>(buf + row * I8_BK + ((q ^ (row & 7)) << 4));
+            }
+#pragma unroll
+            for (int i = 0; i < MI; i++) {
+                const int row = wm * (BM / 2) + i * 32 + (lane & 31);
+                xf[i] = *reinterpret_cast<const i32x4 *>(buf + row * I8_BK + ((q ^ (row & 7)) << 4));
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+                for (int i = 0; i < MI; i++) acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[j], xf[i], acc[j][i], 0, 0, 0);
+        }
+    }
+    __syncthreads();
+    // lane: row lane % 32 of a block, channels 8 g + 4 (lane / 32) + 0..3 in registers 4 g + 0..3
+    constexpr int LD = I8_BN + 16 / sizeof(T);
+    T *out = reinterpret_cast<T *>(lds);
+#pragma unroll
+    for (int i = 0; i < MI; i++) {
+        const int row = wm * (BM / 2) + i * 32 + (lane & 31);
+        const float xs = a.xs[min(m0 + row, a.M - 1)];
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                typedef T out4 __attribute__((ext_vector_type(4)));
+                const int ch = wn * 64 + j * 32 + g * 8 + (lane >> 5) * 4;
+                out4 v;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int n = min(n0 + ch + r, a.N - 1);
+                    v[r] = i8_out<T>(acc[j][i][g * 4 + r], xs, a.ws[n], (const T *)a.bias, n);
+                }
+                *reinterpret_cast<out4 *>(out + row * LD + ch) = v;
+            }
+    }
+    __syncthreads();
+    const int rows = min(BM, a.M - m0), cols = min(I8_BN, a.N - n0);
+    T *y = (T *)a.y + m0 * a.y_stride + n0;
+    constexpr int V = 16 / sizeof(T);
+    if (cols == I8_BN && ((reinterpret_cast<uintptr_t>(y) | (uintptr_t)(a.y_stride * sizeof(T))) & 15) == 0) {
+        for (int i = tid; i < rows * (I8_BN / V); i += 256) {
+            const int row = i / (I8_BN / V), ch = (i - row * (I8_BN / V)) * V;
+            *reinterpret_cast<uint4 *>(y + row * a.y_stride + ch) = *reinterpret_cast<const uint4 *>(out + row * LD + ch);
+        }
+    } else {
+        for (int i = tid; i < rows * I8_BN; i += 256) {
+            const int row = i / I8_BN, ch = i - row * I8_BN;
+            if (ch < cols) y[row * a.y_stride + ch] = out[row * LD + ch];
+        }
+    }
 }
 
 }  // namespace vox

@@ -276,7 +276,18 @@ int check_i8(const char *who, int dtype, int64_t rows, int K) {
     CHECK(K >= 1 && K <= VOX_I8_MAX_K, "%s: K %d (1 to %d)", who, K, VOX_I8_MAX_K);
     return 0;
 }
-int i8_ldq(int K) { return (int)round_up(K, 64); }
+int i8_ldq(int K) { return (int)round_up(K, I8_BK); }
+template <typename T> void launch_quant(const T *x, int64_t stride, int64_t rows, int K, int ldq, int8_t *q, float *scale, hipStream_t s) {
+    constexpr int N = 16 / sizeof(T);
+    const bool wide = K % N == 0 && ldq % N == 0 && stride % N == 0 && aligned(x, 16) && aligned(q, 8);
+    if (wide) hipLaunchKernelGGL((k_quant_rows_i8<T, N>), dim3((unsigned)rows), dim3(256), 0, s, x, stride, K, ldq, q, scale);
+    else hipLaunchKernelGGL((k_quant_rows_i8<T, 1>), dim3((unsigned)rows), dim3(256), 0, s, x, stride, K, ldq, q, scale);
+}
+template <typename T, int BM, int STAGES> void launch_i8_tile(const LinearI8Args &a, hipStream_t s) {
+    const int tm = (a.M + BM - 1) / BM, tn = (a.N + I8_BN - 1) / I8_BN;
+    const unsigned stage = (BM + I8_BN) * I8_BK, out = BM * (I8_BN + 16 / sizeof(T)) * sizeof(T);
+    hipLaunchKernelGGL((k_linear_i8_tile<T, BM, STAGES>), dim3((unsigned)round_up((int64_t)tm * tn, 8)), dim3(256), std::max(STAGES * stage, out), s, a, tm, tn);
+}
 }  // namespace
 extern "C" int vox_hip_quantize_rows_i8(int dtype, const void *x, int64_t row_stride, int64_t rows, int K, int8_t *q, float *scale, int device, void *stream) {
     if (check_i8("vox_hip_quantize_rows_i8", dtype, rows, K)) return -1;
@@ -287,7 +298,7 @@ extern "C" int vox_hip_quantize_rows_i8(int dtype, const void *x, int64_t row_st
     if (!on.ok) return -1;
     by_type(dtype, [&](auto z) {
         typedef decltype(z) T;
-        hipLaunchKernelGGL(k_quant_rows_i8<T>, dim3((unsigned)rows), dim3(256), 0, (hipStream_t)stream, (const T *)x, row_stride, K, K, q, scale);
+        launch_quant<T>((const T *)x, row_stride, rows, K, K, q, scale, (hipStream_t)stream);
     });
     return launched("vox_hip_quantize_rows_i8");
 }
@@ -310,10 +321,19 @@ extern "C" int vox_hip_linear_i8(int dtype, const void *x, int64_t x_stride, int
     int8_t *xq = (int8_t *)ws;
     float *xs = (float *)((char *)ws + round_up(rows * ldq, 256));
     LinearI8Args a{xq, xs, w, w_stride, w_scale, bias, y, y_stride, (int)rows, K, N, ldq};
+    const hipStream_t st = (hipStream_t)stream;
+    const bool wide = K % 16 == 0 && w_stride % 16 == 0 && aligned(w, 16);
     by_type(dtype, [&](auto z) {
         typedef decltype(z) T;
-        hipLaunchKernelGGL(k_quant_rows_i8<T>, dim3((unsigned)rows), dim3(256), 0, (hipStream_t)stream, (const T *)x, x_stride, K, ldq, xq, xs);
-        hipLaunchKernelGGL(k_linear_i8_bytes<T>, dim3((N + 63) / 64, (unsigned)((rows + 63) / 64)), dim3(256), 0, (hipStream_t)stream, a);
+        launch_quant<T>((const T *)x, x_stride, rows, K, ldq, xq, xs, st);
+        const dim3 narrow((N + 15) / 16);
+        if (!wide) hipLaunchKernelGGL(k_linear_i8_bytes<T>, dim3((N + 63) / 64, (unsigned)((rows + 63) / 64)), dim3(256), 0, st, a);
+        else if (rows <= 16) hipLaunchKernelGGL((k_linear_i8_rows<T, 1>), narrow, dim3(64 * I8_ROWS_WAVES), 0, st, a);
+        else if (rows <= 32) hipLaunchKernelGGL((k_linear_i8_rows<T, 2>), narrow, dim3(64 * I8_ROWS_WAVES), 0, st, a);
+        else if (rows <= 64) hipLaunchKernelGGL((k_linear_i8_rows<T, 4>), narrow, dim3(64 * I8_ROWS_WAVES), 0, st, a);
+        else if ((rows + 255) / 256 * ((N + 127) / 128) >= 256) launch_i8_tile<T, 256, 3>(a, st);
+        else if ((rows + 127) / 128 * ((N + 127) / 128) >= 256) launch_i8_tile<T, 128, 2>(a, st);
+        else launch_i8_tile<T, 64, 3>(a, st);
     });
     return launched("vox_hip_linear_i8");
 }
