@@ -301,6 +301,18 @@ def test_token_scores_ties_zeros_and_order():
     check_scores(x[:1].expand(4, V), t[:4], 3)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("top", [1, 7, 64])
+def test_token_scores_hard_orders(dtype, top):
+    """Long rows that rise (every trip brings a new list), fall, are equal throughout, take few values, or hold their largest elements at one end."""
+    V, rng = 40003, np.random.default_rng(top)
+    at = np.arange(V, dtype=np.float32)
+    x = np.stack([at * 1e-3, -at * 1e-3, np.full(V, 2.5), rng.integers(0, 3, V), rng.standard_normal(V), rng.standard_normal(V)]).astype(np.float32)
+    x[4, -70:] += 30
+    x[5, :70] += 30
+    check_scores(dev(x).to(dtype), dev(np.array([[0], [1], [2], [3], [V - 1], [5]], np.int32)), top)
+
+
 def test_token_scores_switched_off_and_broken_rows():
     V = 5000
     rng = np.random.default_rng(9)

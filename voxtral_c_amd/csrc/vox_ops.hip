@@ -223,8 +223,9 @@ extern "C" int vox_hip_tree_attention(const vox_hip_tree_attn_t *a, void *ws, si
 namespace {
 struct ScorePlan { int parts, part_len; int64_t ws; };
 ScorePlan score_plan(int64_t rows, int vocab, int top) {
-    const int step = SC_THREADS * 8;
-    int parts = (int)std::max<int64_t>(1, std::min<int64_t>({SC_MAX_PARTS, 512 / std::max<int64_t>(rows, 1), vocab / (4 * step)}));
+    // Rows are cut until there are about four workgroups per CU, parts down to one trip of a workgroup (SC_UNROLL loads of 16 bytes per thread).
+    const int step = SC_THREADS * 8, trip = SC_THREADS * SC_UNROLL * 4;
+    const int parts = (int)std::max<int64_t>(1, std::min<int64_t>({SC_MAX_PARTS, (1024 + rows / 2) / std::max<int64_t>(rows, 1), vocab / trip}));
     ScorePlan p;
     p.part_len = (int)round_up((vocab + parts - 1) / parts, step);
     p.parts = (vocab + p.part_len - 1) / p.part_len;

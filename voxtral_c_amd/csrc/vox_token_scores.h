@@ -51,20 +51,7 @@ struct ScoreArgs {
     uint64_t *part_top;                      // [rows, parts, top]
 };
 
-// `n` distinct keys in LDS (0 = none) -> the `top` largest in order: a key's place is the number of larger ones.
-__device__ __forceinline__ void top_merge(const uint64_t *keys, int n, int top, uint64_t *out) {
-    for (int i = threadIdx.x; i < top; i += SC_THREADS) out[i] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += SC_THREADS) {
-        const uint64_t key = keys[i];
-        int place = 0;
-        for (int j = 0; j < n; j++) place += keys[j] > key;
-        if (key && place < top) out[place] = key;
-    }
-    __syncthreads();
-}
-
-template <typename T> __device__ __forceinline__ void score_finish(const ScoreArgs &a, int64_t row, const RowSum r, const uint64_t *top) {
+template <typename T> __device__ __forceinline__ void score_finish(const ScoreArgs &a, int64_t row, const RowSum r, uint64_t list) {
     const float log1 = log1pf(r.s);
     auto lp = [&](float x) {
         if (r.m != r.m || r.m == INFINITY) return NAN;
@@ -80,120 +67,301 @@ template <typename T> __device__ __forceinline__ void score_finish(const ScoreAr
         const bool known = id >= 0 && id < a.V;
         a.logprob[row * a.given + i] = known ? lp((float)((const T *)a.logits)[row * a.row_stride + id]) : r.m != r.m ? NAN : -INFINITY;
     }
-    for (int i = threadIdx.x; i < a.top; i += SC_THREADS) {
-        a.top_index[row * a.top + i] = key_index(top[i]);
-        a.top_logprob[row * a.top + i] = lp(key_value(top[i]));
+    if ((int)threadIdx.x < a.top) {                          // (wave 0 holds the list)
+        a.top_index[row * a.top + threadIdx.x] = key_index(list);
+        a.top_logprob[row * a.top + threadIdx.x] = lp(key_value(list));
     }
 }
 
-// Grid (rows * parts).  N elements of T per load.
+__device__ __forceinline__ uint64_t read_lane(uint64_t v, int lane) {
+    return ((uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | (unsigned)__builtin_amdgcn_readlane((int)v, lane);
+}
+// A number that at least k of the wave's 64 ordered numbers reach: the k-th largest, bit by bit, to 20 bits.
+__device__ __forceinline__ unsigned wave_kth(unsigned v, int k) {
+    unsigned t = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 12; bit--) {
+        const unsigned c = t | (1u << bit);
+        if (__popcll(__ballot(v >= c)) >= k) t = c;
+    }
+    return t;
+}
+__device__ __forceinline__ unsigned ordered(float x) { return (unsigned)(score_key(x, 0) >> 32); }
+__device__ __forceinline__ float from_ordered(unsigned u) { return __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u); }
+// The next larger number (-inf and NaN stay what they are as a bound: nothing is below -inf, and fmaxf passes NaN over).
+__device__ __forceinline__ float next_up(float x) { return x == INFINITY || x != x ? x : from_ordered(ordered(x) + 1); }
+
+// The list's lanes one up (lane 0 gets the largest number): v_mov_b32 with wave_shr:1.
+__device__ __forceinline__ uint64_t list_above(uint64_t v) {
+    const unsigned hi = __builtin_amdgcn_update_dpp(-1, (int)(v >> 32), 0x138, 0xf, 0xf, false);
+    const unsigned lo = __builtin_amdgcn_update_dpp(-1, (int)v, 0x138, 0xf, 0xf, false);
+    return ((uint64_t)hi << 32) | lo;
+}
+// The value of lane ^ X: DPP within rows of 16, v_permlane*_swap across them (a fraction of the latency of a trip through ds_bpermute).
+template <int X> __device__ __forceinline__ unsigned lane_xor(unsigned v) {
+    if constexpr (X == 1) return __builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true);              // quad_perm 1 0 3 2
+    else if constexpr (X == 2) return __builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true);         // quad_perm 2 3 0 1
+    else if constexpr (X == 4) return __builtin_amdgcn_update_dpp(0, __builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true), 0x1B, 0xf, 0xf, true);   // half mirror, quad mirror
+    else if constexpr (X == 8) return __builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, true);        // row_ror 8
+    else if constexpr (X == 15) return __builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true);       // row_mirror
+    else if constexpr (X == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return (threadIdx.x & 16) ? r[0] : r[1];
+    } else {
+        static_assert(X == 32, "");
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return (threadIdx.x & 32) ? r[0] : r[1];
+    }
+}
+template <int X> __device__ __forceinline__ uint64_t lane_xor64(uint64_t v) {
+    return ((uint64_t)lane_xor<X>((unsigned)(v >> 32)) << 32) | lane_xor<X>((unsigned)v);
+}
+// One step of a bitonic network: of lanes l and l ^ X, the one with bit X clear keeps the larger key if `falling`.
+template <int X> __device__ __forceinline__ uint64_t bitonic_step(uint64_t v, bool falling) {
+    const uint64_t other = lane_xor64<X>(v);
+    return (((threadIdx.x & X) == 0) == falling) == (other > v) ? other : v;
+}
+template <int X> __device__ __forceinline__ uint64_t bitonic_merge(uint64_t v, bool falling) {
+    v = bitonic_step<X>(v, falling);
+    if constexpr (X > 1) v = bitonic_merge<X / 2>(v, falling);
+    return v;
+}
+// n keys in the lanes (0 behind them), falling afterwards.
+__device__ __forceinline__ uint64_t bitonic_sort(uint64_t v, int n) {
+    const int lane = threadIdx.x & 63;
+    if (n > 1) v = bitonic_merge<1>(v, (lane & 2) == 0);
+    if (n > 2) v = bitonic_merge<2>(v, (lane & 4) == 0);
+    if (n > 4) v = bitonic_merge<4>(v, (lane & 8) == 0);
+    if (n > 8) v = bitonic_merge<8>(v, (lane & 16) == 0);
+    if (n > 16) v = bitonic_merge<16>(v, (lane & 32) == 0);
+    if (n > 32) v = bitonic_merge<32>(v, true);
+    return v;
+}
+// The 64 largest of two falling lists, falling.
+__device__ __forceinline__ uint64_t list_join(uint64_t list, uint64_t more) {
+    more = lane_xor64<32>(lane_xor64<16>(lane_xor64<15>(more)));
+    return bitonic_merge<32>(list > more ? list : more, true);
+}
+// The waves' lists -> wave 0's list; `keys`: [SC_WAVES][64] in LDS.
+__device__ __forceinline__ uint64_t waves_join(uint64_t list, uint64_t *keys) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    keys[threadIdx.x] = list;
+    __syncthreads();
+#pragma unroll
+    for (int half = SC_WAVES / 2; half > 0; half >>= 1) {
+        if (wave < half) keys[threadIdx.x] = list = list_join(list, keys[(wave + half) * 64 + lane]);
+        __syncthreads();
+    }
+    return list;
+}
+
+__device__ __forceinline__ float wave_max_dpp(float v) {
+    v = fmaxf(v, __uint_as_float(lane_xor<1>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(lane_xor<2>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(lane_xor<4>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(lane_xor<8>(__float_as_uint(v))));
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// Grid (rows * parts).  N elements of T per load.  A wave's maximum is one number for all its lanes: it grows about ln(trips) times per row, and
+// only then are the sums rescaled (a maximum per lane grows in some lane on almost every load: 113 -> see below).
 template <typename T, int N> __global__ __launch_bounds__(SC_THREADS) void k_token_scores(ScoreArgs a) {
+    constexpr int U = N == 8 ? 2 : SC_UNROLL;
     __shared__ RowSum sums[SC_WAVES];
-    __shared__ uint64_t keys[SC_WAVES * SC_TOP], best[SC_TOP];
+    __shared__ uint64_t pending[SC_WAVES][128];
+    // Of each wave's list as it last was: its `top`-th value and its ceil(top / SC_WAVES)-th.  Hints: results do not depend on when they are seen.
+    __shared__ float bar_full[SC_WAVES], bar_share[SC_WAVES];
     const int64_t row = blockIdx.x / a.parts;
     const int part = blockIdx.x - (int)row * a.parts, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (tid < SC_WAVES) bar_full[tid] = bar_share[tid] = -INFINITY;
+    __syncthreads();
     const T *x = (const T *)a.logits + row * a.row_stride;
     const int begin = part * a.part_len, end = min(begin + a.part_len, a.V);
-    RowSum r{-INFINITY, -1.f, 0.f};
-    uint64_t list = 0, last = 0;                             // this lane's entry; the list's `top`-th (uniform)
-    float bar = NAN;                                         // value of `last` (NaN: the list is not full)
-    for (int i0 = begin; i0 < end; i0 += SC_THREADS * N * SC_UNROLL) {
-        float f[SC_UNROLL][N];
+    float m = -INFINITY, s = 0.f, t = 0.f;                   // RowSum of the wave, s and t by lanes; the maximum's own term is left out of s
+    uint64_t *mine = pending[wave];
+    uint64_t list = 0, last = 0;                             // this lane's entry; the list's `top`-th (uniform, 0: the list is not full)
+    float limit = -INFINITY;                                 // nothing below it can stay
+    constexpr int TRIP = SC_THREADS * N * U;
+    typedef T vec __attribute__((ext_vector_type(N)));
+    vec raw[U];                                      // the next trip's elements, on their way while a trip is worked on
+    auto fetch = [&](int i0) {
+        if (i0 + TRIP <= end) {
 #pragma unroll
-        for (int u = 0; u < SC_UNROLL; u++) {
-            const int at = i0 + (u * SC_THREADS + tid) * N;
-            if (at + N <= end) load_vec<T, N>(f[u], x + at);
-            else
-#pragma unroll
-                for (int j = 0; j < N; j++) f[u][j] = at + j < end ? (float)x[at + j] : -INFINITY;
+            for (int u = 0; u < U; u++) raw[u] = *reinterpret_cast<const vec *>(x + i0 + (u * SC_THREADS + tid) * N);
         }
+    };
+    fetch(begin);
+    for (int i0 = begin; i0 < end; i0 += TRIP) {
+        float f[U][N], group[U * N / 4 > 0 ? U * N / 4 : 1], most = -INFINITY;       // group: maxima of four elements each (N = 1: of all)
+        if (i0 + TRIP <= end) {
 #pragma unroll
-        for (int u = 0; u < SC_UNROLL; u++) {
-            float vm = f[u][0];
+            for (int u = 0; u < U; u++)
 #pragma unroll
-            for (int j = 1; j < N; j++) vm = fmaxf(vm, f[u][j]);
-            if (vm > r.m) {
-                const float l = 1.f + r.s, d = r.m - vm, e = r.m == -INFINITY ? 0.f : exp_fast(d);
-                r.t = e == 0.f ? 0.f : e * (r.t + d * l);
-                r.s = e * l;
-                r.m = vm;
-                bool own = true;                             // the maximum's own term, once
+                for (int j = 0; j < N; j++) f[u][j] = (float)raw[u][j];
+        } else {
 #pragma unroll
-                for (int j = 0; j < N; j++) {
-                    const float dj = f[u][j] - vm, ej = exp_fast(dj);
-                    if (own && f[u][j] == vm) { own = false; continue; }
-                    r.s += ej;
-                    r.t += ej * fmaxf(dj, -200.f);           // (e^-inf * -inf is 0 here)
-                }
-            } else {
-                const float base = r.m == -INFINITY ? 0.f : r.m;
+            for (int u = 0; u < U; u++)
 #pragma unroll
                 for (int j = 0; j < N; j++) {
-                    const float dj = f[u][j] - base, ej = exp_fast(dj);
-                    r.s += ej;
-                    r.t += ej * fmaxf(dj, -200.f);
+                    const int at = i0 + (u * SC_THREADS + tid) * N + j;
+                    f[u][j] = at < end ? (float)x[at] : -INFINITY;
                 }
+        }
+        fetch(i0 + TRIP);
+#pragma unroll
+        for (int g = 0; g < U * N / 4; g++) {
+            const int u = g * 4 / N, j = g * 4 % N;          // (N = 1: the four loads)
+            group[g] = N >= 4 ? fmaxf(fmaxf(f[u][j], f[u][(j + 1) % N]), fmaxf(f[u][(j + 2) % N], f[u][(j + 3) % N]))
+                              : fmaxf(fmaxf(f[u % U][0], f[(u + 1) % U][0]), fmaxf(f[(u + 2) % U][0], f[(u + 3) % U][0]));
+            most = fmaxf(most, group[g]);
+        }
+        const float peak = wave_max_dpp(most);
+        if (peak > m) {
+            if (m != -INFINITY) {                            // the old maximum's own term joins the others
+                const float d = m - peak, e = exp_fast(d);
+                s += lane == 0 ? 1.f : 0.f;
+                t = e * (t + d * s);
+                s *= e;
             }
+            m = peak;
+            bool own = (__ffsll((unsigned long long)__ballot(most == peak)) - 1) == lane;      // the new one's, once
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    const bool skip = own && f[u][j] == m;
+                    const float d = f[u][j] - m, e = skip ? 0.f : exp_fast(d);
+                    own = own && !skip;
+                    s += e;
+                    t += e * fmaxf(d, -200.f);               // (e^-inf * -inf is 0 here)
+                }
+        } else {
+            const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    const float d = f[u][j] - base, e = exp_fast(d);
+                    s += e;
+                    t += e * fmaxf(d, -200.f);
+                }
         }
         if (a.top > 0) {
-            // An element that only equals the bar comes behind the elements of earlier trips that put it there: strictly larger ones go on.
-            const float limit = bar;
+            // Candidates: what reaches the limit, and NaN, which the sum shows.  The limit comes from this wave's list (strictly above its `top`-th: an
+            // equal element of a later trip comes behind it), from the other waves' lists (their `top`-th; and the smallest of all waves'
+            // ceil(top / waves)-th, which are `top` elements or more together), and, where many lanes have a candidate, from a number that `top` of
+            // the lanes' largest reach.
+            const bool nan = __any(s != s);
+            if (nan || !(peak < limit)) {
+                float all = bar_share[0];
 #pragma unroll
-            for (int u = 0; u < SC_UNROLL; u++) {
-                bool any = false;
+                for (int w = 0; w < SC_WAVES; w++) {
+                    limit = fmaxf(limit, bar_full[w]);
+                    all = fminf(all, bar_share[w]);
+                }
+                limit = fmaxf(limit, all);
+            }
+            if (nan || !(peak < limit)) {
+                int waiting = 0;                             // keys in `mine` that are not in the list yet
+                float here = limit;                          // within this trip (equal elements may still come first)
+                const uint64_t lanes = __ballot(nan || !(most < here));
+                if (__popcll(lanes) >= max(a.top, 16)) here = fmaxf(here, from_ordered(wave_kth(nan ? 0x007fffffu : ordered(most), a.top)));
 #pragma unroll
-                for (int j = 0; j < N; j++) any |= !(f[u][j] <= limit);
-                if (__ballot(any) == 0) continue;
-                const int at = i0 + (u * SC_THREADS + tid) * N;
+                for (int g = 0; g < U * N / 4; g++) {
+                    if (__ballot(nan || !(group[g] < here)) == 0) continue;
 #pragma unroll
-                for (int j = 0; j < N; j++) {
-                    uint64_t todo = __ballot(!(f[u][j] <= limit) && at + j < end);
-                    const uint64_t mine = score_key(f[u][j], at + j);
-                    while (todo) {
-                        const int src = __ffsll((unsigned long long)todo) - 1;
-                        todo &= todo - 1;
-                        const uint64_t key = ((uint64_t)__builtin_amdgcn_readlane((int)(mine >> 32), src) << 32) |
-                                             (unsigned)__builtin_amdgcn_readlane((int)mine, src);
-                        if (key <= last) continue;
-                        const uint64_t above = ((uint64_t)(unsigned)__shfl_up((int)(list >> 32), 1, 64) << 32) | (unsigned)__shfl_up((int)list, 1, 64);
-                        list = list > key ? list : (lane == 0 || above > key) ? key : above;
-                        last = ((uint64_t)__builtin_amdgcn_readlane((int)(list >> 32), a.top - 1) << 32) |
-                               (unsigned)__builtin_amdgcn_readlane((int)list, a.top - 1);
+                    for (int i = 0; i < 4; i++) {
+                        const int u = (g * 4 + i) / N, j = (g * 4 + i) % N, at = i0 + (u * SC_THREADS + tid) * N + j;
+                        const bool pass = !(f[u][j] < here) && at < end;
+                        const uint64_t todo = __ballot(pass);
+                        if (todo == 0) continue;
+                        if (pass) mine[waiting + __builtin_amdgcn_mbcnt_hi((unsigned)(todo >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)todo, 0))] = score_key(f[u][j], at);
+                        waiting += __popcll(todo);
+                        if (waiting >= 64) {
+                            list = list_join(list, bitonic_sort(mine[lane], 64));
+                            waiting -= 64;
+                            if (lane < waiting) mine[lane] = mine[64 + lane];
+                            last = read_lane(list, a.top - 1);
+                            if (last) here = fmaxf(here, key_value(last));
+                        }
                     }
                 }
+                if (waiting > 4) list = list_join(list, bitonic_sort(lane < waiting ? mine[lane] : 0, waiting));
+                else
+                    for (int i = 0; i < waiting; i++) {      // a few: one by one (a join is nine steps of the network)
+                        const uint64_t key = mine[i], above = list_above(list);
+                        list = list > key ? list : above > key ? key : above;
+                    }
+                last = read_lane(list, a.top - 1);
+                if (last) {
+                    const float bar = key_value(last), share = key_value(read_lane(list, (a.top + SC_WAVES - 1) / SC_WAVES - 1));
+                    limit = fmaxf(limit, next_up(bar));
+                    if (lane == 0) { bar_full[wave] = bar; bar_share[wave] = share == share ? share : INFINITY; }
+                }
             }
-            bar = last ? key_value(last) : NAN;
         }
     }
-    if (r.s != r.s && r.m != INFINITY) r.m = NAN;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const RowSum b{__shfl_xor(r.m, o, 64), __shfl_xor(r.s, o, 64), __shfl_xor(r.t, o, 64)};
-        r = row_join(r, b);
-    }
+    s = wave_sum(s);
+    t = wave_sum(t);
+    RowSum r{s != s && m != INFINITY ? NAN : m, m == -INFINITY ? -1.f : s, t};
     if (lane == 0) sums[wave] = r;
-    if (lane < a.top) keys[wave * a.top + lane] = list;
     __syncthreads();
     r = sums[0];
 #pragma unroll
     for (int w = 1; w < SC_WAVES; w++) r = row_join(r, sums[w]);
-    top_merge(keys, SC_WAVES * a.top, a.top, best);
-    if (a.parts == 1) { score_finish<T>(a, row, r, best); return; }
+    if (a.top > 0) list = waves_join(list, &pending[0][0]);
+    if (a.parts == 1) { score_finish<T>(a, row, r, list); return; }
     if (tid == 0) a.part_sum[row * a.parts + part] = r;
-    for (int i = tid; i < a.top; i += SC_THREADS) a.part_top[(row * a.parts + part) * a.top + i] = best[i];
+    if (tid < a.top) a.part_top[(row * a.parts + part) * a.top + tid] = list;
 }
 
 // Grid (rows): joins the parts of a row.
 constexpr int SC_MAX_PARTS = 32;
 template <typename T> __global__ __launch_bounds__(SC_THREADS) void k_token_scores_join(ScoreArgs a) {
-    __shared__ uint64_t keys[SC_MAX_PARTS * SC_TOP], best[SC_TOP];
+    __shared__ uint64_t pending[SC_WAVES][128];
     const int64_t row = blockIdx.x;
-    for (int i = threadIdx.x; i < a.parts * a.top; i += SC_THREADS) keys[i] = a.part_top[row * a.parts * a.top + i];
-    RowSum r = a.part_sum[row * a.parts];
-    for (int p = 1; p < a.parts; p++) r = row_join(r, a.part_sum[row * a.parts + p]);
-    __syncthreads();
-    top_merge(keys, a.parts * a.top, a.top, best);
-    score_finish<T>(a, row, r, best);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    RowSum r{-INFINITY, -1.f, 0.f};
+    if (lane < a.parts) r = a.part_sum[row * a.parts + lane];
+#pragma unroll
+    for (int o = 1; o < SC_MAX_PARTS; o <<= 1) {
+        const RowSum b{__shfl_xor(r.m, o, 64), __shfl_xor(r.s, o, 64), __shfl_xor(r.t, o, 64)};
+        r = row_join(r, b);
+    }
+    r = RowSum{__shfl(r.m, 0, 64), __shfl(r.s, 0, 64), __shfl(r.t, 0, 64)};
+    uint64_t list = 0;
+    if (a.top > 0) {
+        // The parts' entries number ceil(top / parts) are `top` keys or more together: the smallest of them bounds from below what can stay.
+        const uint64_t *keys = a.part_top + row * a.parts * a.top;
+        uint64_t bound = lane < a.parts ? keys[lane * a.top + (a.top + a.parts - 1) / a.parts - 1] : ~0ull;
+#pragma unroll
+        for (int o = 1; o < SC_MAX_PARTS; o <<= 1) {
+            const uint64_t b = ((uint64_t)(unsigned)__shfl_xor((int)(bound >> 32), o, 64) << 32) | (unsigned)__shfl_xor((int)bound, o, 64);
+            bound = min(bound, b);
+        }
+        bound = read_lane(bound, 0);
+        uint64_t *mine = pending[wave];
+        int waiting = 0;
+        for (int i = wave * 64; i < a.parts * a.top; i += SC_THREADS) {
+            const uint64_t key = i + lane < a.parts * a.top ? keys[i + lane] : 0;
+            const bool pass = key && key >= bound;
+            const uint64_t todo = __ballot(pass);
+            if (pass) mine[waiting + __builtin_amdgcn_mbcnt_hi((unsigned)(todo >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)todo, 0))] = key;
+            waiting += __popcll(todo);
+            if (waiting >= 64) {
+                list = list_join(list, bitonic_sort(mine[lane], 64));
+                waiting -= 64;
+                if (lane < waiting) mine[lane] = mine[64 + lane];
+            }
+        }
+        if (waiting) list = list_join(list, bitonic_sort(lane < waiting ? mine[lane] : 0, waiting));
+        __syncthreads();
+        list = waves_join(list, &pending[0][0]);
+    }
+    score_finish<T>(a, row, r, list);
 }
 
 }  // namespace vox

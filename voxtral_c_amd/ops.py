@@ -50,42 +50,46 @@ def _error(who):
     raise VoxError(f"{who}: {hip.vox_hip_last_error().decode()}")
 
 
-def _float_args(who, shapes):
-    """`shapes`: (name, tensor, shape).  One floating type of _DTYPES, the given shapes, a contiguous last dimension; returns the type's number."""
-    dtype = shapes[0][1].dtype
-    number = _DTYPES.get(dtype)
-    if number is None:
-        raise ValueError(f"{who}: {shapes[0][0]} is {dtype}: float32, bfloat16 or float16 are supported")
-    for name, t, shape in shapes:
-        if t.dtype != dtype:
-            raise ValueError(f"{who}: {name} is {t.dtype}, {shapes[0][0]} is {dtype}: one type is needed")
-        if t.shape != shape:
-            raise ValueError(f"{who}: {name} has the shape {tuple(t.shape)}: {tuple(shape)} is needed")
-        if t.stride(-1) != 1 and t.shape[-1] > 1:
+def _float_args(who, *named):
+    """`named`: name, tensor, shape, name, .. .  One floating type of _DTYPES, the given shapes, a contiguous last dimension; returns the type's number."""
+    dtype, grad = named[1].dtype, torch.is_grad_enabled()
+    for i in range(0, len(named), 3):
+        t, shape = named[i + 1], named[i + 2]
+        if t.dtype is not dtype or t.shape != shape or (t.stride(-1) != 1 and shape[-1] > 1) or (grad and t.requires_grad) or dtype not in _DTYPES:
+            name = named[i]
+            if dtype not in _DTYPES:
+                raise ValueError(f"{who}: {name} is {dtype}: float32, bfloat16 or float16 are supported")
+            if t.dtype != dtype:
+                raise ValueError(f"{who}: {name} is {t.dtype}, {named[0]} is {dtype}: one type is needed")
+            if t.shape != shape:
+                raise ValueError(f"{who}: {name} has the shape {tuple(t.shape)}: {tuple(shape)} is needed")
+            if t.requires_grad and grad:
+                raise ValueError(f"{who}: {name} needs gradients: there is no backward pass (use torch.no_grad())")
             raise ValueError(f"{who}: the last dimension of {name} is not contiguous")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError(f"{who}: {name} needs gradients: there is no backward pass (use torch.no_grad())")
-    return number
+    return _DTYPES[dtype]
 
 
 def _table(who, name, t, shape, dtype=_I32):
-    if t.dtype != dtype or t.shape != shape:
+    if t.dtype is not dtype or t.shape != shape:
         raise ValueError(f"{who}: {name} is {t.dtype} {tuple(t.shape)}: {dtype} {tuple(shape)} is needed")
     return t if t.is_contiguous() else t.contiguous()
 
 
 def _device(who, *tensors):
-    d = tensors[0].device
-    if d.type != "cuda":
-        raise ValueError(f"{who}: tensors are on {d}: a GPU is needed (there is no CPU path)")
+    """The tensors' one GPU, as its number."""
+    d = tensors[0].get_device()
     for t in tensors:
-        if t.device != d:
-            raise ValueError(f"{who}: tensors on {d} and {t.device}: one device is needed")
+        if t.get_device() != d or d < 0 or not t.is_cuda:
+            raise ValueError(f"{who}: tensors on {tensors[0].device} and {t.device}: " + ("one device is needed" if t.device != tensors[0].device else
+                                                                                            "a GPU is needed (there is no CPU path)"))
     return d
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # (what current_stream gives, without the object around it)
+
+
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(device) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
 
 
 def _nodes(who, shape):
@@ -103,9 +107,9 @@ def tree_plan(parents, n_nodes=None):
     if n_nodes is not None:
         n_nodes = _table(who, "n_nodes", n_nodes, (B,))
     d = _device(who, parents, *(() if n_nodes is None else (n_nodes,)))
-    ancestors = torch.empty((B, T, (T + 63) // 64), dtype=torch.int64, device=d)
-    depth = torch.empty((B, T), dtype=_I32, device=d)
-    if hip.vox_hip_tree_plan(parents.data_ptr(), None if n_nodes is None else n_nodes.data_ptr(), B, T, ancestors.data_ptr(), depth.data_ptr(), d.index, _stream(d)):
+    ancestors = parents.new_empty((B, T, (T + 63) // 64), dtype=torch.int64)
+    depth = parents.new_empty((B, T))
+    if hip.vox_hip_tree_plan(parents.data_ptr(), None if n_nodes is None else n_nodes.data_ptr(), B, T, ancestors.data_ptr(), depth.data_ptr(), d, _stream(d)):
         _error(who)
     return ancestors, depth
 
@@ -124,19 +128,19 @@ def tree_attention(q, k, v, k_cache, v_cache, cache_len, ancestors, depth, scale
     if Hk < 1 or H % Hk or not 1 <= D <= 256 or cap < 1:
         raise ValueError(f"{who}: {H} heads over {Hk} kv heads of {D} (at most 256), a cache of {cap} rows")
     cache = (B, cap, Hk, D)
-    number = _float_args(who, (("q", q, (B, T, H, D)), ("k", k, (B, T, Hk, D)), ("v", v, (B, T, Hk, D)), ("k_cache", k_cache, cache), ("v_cache", v_cache, cache)))
+    number = _float_args(who, "q", q, q.shape, "k", k, (B, T, Hk, D), "v", v, (B, T, Hk, D), "k_cache", k_cache, cache, "v_cache", v_cache, cache)
     cache_len = _table(who, "cache_len", cache_len, (B,))
     ancestors = _table(who, "ancestors", ancestors, (B, T, (T + 63) // 64), torch.int64)
     depth = _table(who, "depth", depth, (B, T))
     d = _device(who, q, k, v, k_cache, v_cache, cache_len, ancestors, depth)
-    out = torch.empty((B, T, H, D), dtype=q.dtype, device=d)
-    lse = torch.empty((B, T, H), dtype=torch.float32, device=d) if return_lse else None
+    out = q.new_empty((B, T, H, D))
+    lse = q.new_empty((B, T, H), dtype=torch.float32) if return_lse else None
     args = _ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), cache_len.data_ptr(), ancestors.data_ptr(), depth.data_ptr(),
                       out.data_ptr(), 0 if lse is None else lse.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *k_cache.stride()[:3], *v_cache.stride()[:3],
                       T * H * D, H * D, D, number, B, T, H, Hk, D, cap, max(-1, min(int(window), 0x7fffffff)), D ** -0.5 if scale is None else scale, 0)
     need = hip.vox_hip_tree_attention_workspace(args)
-    ws = torch.empty(need, dtype=torch.uint8, device=d) if need > 0 else None
-    if need < 0 or hip.vox_hip_tree_attention(args, None if ws is None else ws.data_ptr(), need, d.index, _stream(d)):
+    ws = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
+    if need < 0 or hip.vox_hip_tree_attention(args, None if ws is None else ws.data_ptr(), need, d, _stream(d)):
         _error(who)
     return (out, lse) if return_lse else out
 
@@ -150,14 +154,14 @@ def tree_accept(tokens, choices, root_choice, parents, ancestors, depth, cache_l
     B, T = tokens.shape if tokens.dim() == 2 else (-1, -1)
     if T == 0:
         raise ValueError(f"{who}: no nodes")
-    tokens, choices, parents, depth = (_table(who, n, t, (B, T)) for n, t in (("tokens", tokens), ("choices", choices), ("parents", parents), ("depth", depth)))
+    tokens, choices = _table(who, "tokens", tokens, (B, T)), _table(who, "choices", choices, (B, T))
+    parents, depth = _table(who, "parents", parents, (B, T)), _table(who, "depth", depth, (B, T))
     root_choice, cache_len = _table(who, "root_choice", root_choice, (B,)), _table(who, "cache_len", cache_len, (B,))
     ancestors = _table(who, "ancestors", ancestors, (B, T, (T + 63) // 64), torch.int64)
     d = _device(who, tokens, choices, root_choice, parents, ancestors, depth, cache_len)
-    path = torch.empty((B, T), dtype=_I32, device=d)
-    n, after, new_len = torch.empty((3, B), dtype=_I32, device=d)
+    path, n, after, new_len = tokens.new_empty((B, T)), tokens.new_empty((B,)), tokens.new_empty((B,)), tokens.new_empty((B,))
     if hip.vox_hip_tree_accept(tokens.data_ptr(), choices.data_ptr(), root_choice.data_ptr(), parents.data_ptr(), ancestors.data_ptr(), depth.data_ptr(),
-                               cache_len.data_ptr(), B, T, path.data_ptr(), n.data_ptr(), after.data_ptr(), new_len.data_ptr(), d.index, _stream(d)):
+                               cache_len.data_ptr(), B, T, path.data_ptr(), n.data_ptr(), after.data_ptr(), new_len.data_ptr(), d, _stream(d)):
         _error(who)
     return path, n, after, new_len
 
@@ -175,7 +179,7 @@ def tree_commit(k, v, k_cache, v_cache, path, n_accepted, cache_len):
     _nodes(who, k.shape[1:])
     if cap < T:
         raise ValueError(f"{who}: a ring of {cap} rows does not hold a path of {T} nodes")
-    number = _float_args(who, (("k", k, (L, B, T, Hk, D)), ("v", v, (L, B, T, Hk, D)), ("k_cache", k_cache, (L, B, cap, Hk, D)), ("v_cache", v_cache, (L, B, cap, Hk, D))))
+    number = _float_args(who, "k", k, k.shape, "v", v, k.shape, "k_cache", k_cache, (L, B, cap, Hk, D), "v_cache", v_cache, (L, B, cap, Hk, D))
     path, n_accepted, cache_len = _table(who, "path", path, (B, T)), _table(who, "n_accepted", n_accepted, (B,)), _table(who, "cache_len", cache_len, (B,))
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
         if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
@@ -183,7 +187,7 @@ def tree_commit(k, v, k_cache, v_cache, path, n_accepted, cache_len):
     d = _device(who, k, v, k_cache, v_cache, path, n_accepted, cache_len)
     if hip.vox_hip_tree_commit(number, L, B, T, Hk, D, cap, k.data_ptr(), _Strides(*k.stride()[:4]), v.data_ptr(), _Strides(*v.stride()[:4]),
                                k_cache.data_ptr(), _Strides(*k_cache.stride()[:4]), v_cache.data_ptr(), _Strides(*v_cache.stride()[:4]),
-                               path.data_ptr(), n_accepted.data_ptr(), cache_len.data_ptr(), d.index, _stream(d)):
+                               path.data_ptr(), n_accepted.data_ptr(), cache_len.data_ptr(), d, _stream(d)):
         _error(who)
 
 
@@ -198,7 +202,7 @@ def token_scores(logits, tokens=None, top=0):
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"{who}: logits have the shape {tuple(logits.shape)}: [rows, vocab] is needed")
     R, V = logits.shape
-    number = _float_args(who, (("logits", logits, (R, V)),))
+    number = _float_args(who, "logits", logits, logits.shape)
     if not 0 <= top <= min(MAX_TOP, V):
         raise ValueError(f"{who}: top {top} of {V} (at most {MAX_TOP})")
     shape = (R, 0)
@@ -206,16 +210,14 @@ def token_scores(logits, tokens=None, top=0):
         shape = (R,) if tokens.dim() == 1 else (R, tokens.shape[-1])
         tokens = _table(who, "tokens", tokens, shape)
     d = _device(who, logits) if tokens is None else _device(who, logits, tokens)
-    logprob = torch.empty(shape, dtype=torch.float32, device=d)
-    entropy, lse = torch.empty((2, R), dtype=torch.float32, device=d)
-    top_index = torch.empty((R, top), dtype=_I32, device=d)
-    top_logprob = torch.empty((R, top), dtype=torch.float32, device=d)
+    new, f32 = logits.new_empty, torch.float32
+    logprob, entropy, lse, top_index, top_logprob = new(shape, dtype=f32), new((R,), dtype=f32), new((R,), dtype=f32), new((R, top), dtype=_I32), new((R, top), dtype=f32)
     need = hip.vox_hip_token_scores_workspace(number, R, V, top)
-    ws = torch.empty(need, dtype=torch.uint8, device=d) if need > 0 else None
+    ws = new(need, dtype=torch.uint8) if need > 0 else None
     given = 0 if tokens is None else 1 if len(shape) == 1 else shape[1]
     if need < 0 or hip.vox_hip_token_scores(number, logits.data_ptr(), logits.stride(0), R, V, None if tokens is None else tokens.data_ptr(), given, top,
                                             logprob.data_ptr(), entropy.data_ptr(), lse.data_ptr(), top_index.data_ptr(), top_logprob.data_ptr(),
-                                            None if ws is None else ws.data_ptr(), max(need, 0), d.index, _stream(d)):
+                                            None if ws is None else ws.data_ptr(), need, d, _stream(d)):
         _error(who)
     return TokenScores(logprob, entropy, lse, top_index, top_logprob)
 
@@ -226,11 +228,10 @@ def quantize_rows_i8(x):
     who = "quantize_rows_i8"
     if x.dim() != 2 or not 1 <= x.shape[1] <= 131072:
         raise ValueError(f"{who}: x has the shape {tuple(x.shape)}: [rows, K] with K of 1 to 131072 is needed")
-    number = _float_args(who, (("x", x, x.shape),))
+    number = _float_args(who, "x", x, x.shape)
     d = _device(who, x)
-    q = torch.empty(x.shape, dtype=torch.int8, device=d)
-    scale = torch.empty(x.shape[0], dtype=torch.float32, device=d)
-    if hip.vox_hip_quantize_rows_i8(number, x.data_ptr(), x.stride(0), x.shape[0], x.shape[1], q.data_ptr(), scale.data_ptr(), d.index, _stream(d)):
+    q, scale = x.new_empty(x.shape, dtype=torch.int8), x.new_empty(x.shape[0], dtype=torch.float32)
+    if hip.vox_hip_quantize_rows_i8(number, x.data_ptr(), x.stride(0), x.shape[0], x.shape[1], q.data_ptr(), scale.data_ptr(), d, _stream(d)):
         _error(who)
     return q, scale
 
@@ -243,16 +244,15 @@ def linear_i8(x, w, w_scale, bias=None):
         raise ValueError(f"{who}: x has the shape {tuple(x.shape)}, w {tuple(w.shape)}: [rows, K] and [outputs, K] with K of 1 to 131072 are needed")
     M, K = x.shape
     N = w.shape[0]
-    floats = (("x", x, (M, K)),) if bias is None else (("x", x, (M, K)), ("bias", bias, (N,)))
-    number = _float_args(who, floats)
+    number = _float_args(who, "x", x, x.shape) if bias is None else _float_args(who, "x", x, x.shape, "bias", bias, (N,))
     if w.dtype != torch.int8 or w.shape[1] != K or (w.stride(1) != 1 and K > 1):
         raise ValueError(f"{who}: w is {w.dtype} {tuple(w.shape)}: int8 {(N, K)} with contiguous rows is needed")
     w_scale = _table(who, "w_scale", w_scale, (N,), torch.float32)
     d = _device(who, x, w, w_scale, *(() if bias is None else (bias,)))
-    y = torch.empty((M, N), dtype=x.dtype, device=d)
+    y = x.new_empty((M, N))
     need = hip.vox_hip_linear_i8_workspace(number, M, K, N)
-    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=d)
+    ws = x.new_empty(max(need, 1), dtype=torch.uint8)
     if need < 0 or hip.vox_hip_linear_i8(number, x.data_ptr(), x.stride(0), M, K, N, w.data_ptr(), w.stride(0), w_scale.data_ptr(),
-                                         None if bias is None else bias.data_ptr(), y.data_ptr(), N, ws.data_ptr(), need, d.index, _stream(d)):
+                                         None if bias is None else bias.data_ptr(), y.data_ptr(), N, ws.data_ptr(), need, d, _stream(d)):
         _error(who)
     return y
