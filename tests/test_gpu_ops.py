@@ -126,6 +126,7 @@ ATTN = [
     (1, 65, 6, 2, 64, 100, [37], 0), (1, 256, 8, 2, 64, 40, [40], 9), (4, 5, 3, 3, 96, 70, [70, 69, 1, 33], 0), (1, 33, 8, 1, 128, 129, [128], 0),
     (2, 3, 4, 2, 256, 50, [49, 50], 0), (2, 3, 5, 5, 33, 20, [44, 7], 11), (1, 4, 4, 2, 1, 9, [9], 0), (1, 17, 12, 4, 80, 64, [64], 1), (1, 6, 16, 1, 192, 90, [77], 0),
     (2, 3, 8, 2, 128, 1500, [1500, 1111], 0), (1, 16, 4, 1, 64, 2100, [2099], 2000),
+    (16, 12, 32, 8, 64, 1000, [1000, 612, 999], 0), (16, 24, 32, 8, 128, 700, [3000, 700, 350, 64], 600), (32, 2, 32, 16, 128, 900, [900, 31, 1800], 0),
 ]
 
 
@@ -155,10 +156,11 @@ def test_tree_attention_strides(dtype):
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("D", [64, 128, 40])
-def test_tree_attention_ignores_what_is_masked(dtype, D):
+@pytest.mark.parametrize("H", [4, 16, 24])
+def test_tree_attention_ignores_what_is_masked(dtype, D, H):
     """NaN, infinities and the type's largest values in rows that nobody (or not everybody) may see."""
     B, T, window, cap = 2, 6, 20, 40
-    c = attn_case(11, dtype, B, T, 4, 2, D, cap, [33, 9])
+    c = attn_case(11, dtype, B, T, H, 2, D, cap, [33, 9])
     clean = check_attn(c, window)
     for bad in (math.nan, math.inf, -math.inf, torch.finfo(dtype).max, torch.finfo(dtype).min):
         x = {**c, **{n: c[n].clone() for n in ("k", "v", "k_cache", "v_cache")}}
@@ -187,6 +189,36 @@ def test_tree_attention_any_mask(dtype):
     c["ancestors"] = a
     out, lse = check_attn(c)
     assert (out[0, 0] == 0).all() and torch.isneginf(lse[0, 0]).all() and torch.isfinite(lse[1, 0]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("H", [2, 40])
+def test_tree_attention_passes_on_what_is_seen(dtype, H):
+    """An infinite value in the tree or at a window's edge reaches the rows that see it, with its sign, and nobody else; NaN and both signs give NaN."""
+    window, D, T = 12, 64, 3
+    c = attn_case(13, dtype, 1, T, H, 2, D, 16, [14], shorter=False)
+    c["ancestors"] = dev(np.array([[[1], [3], [5]]], np.int64))        # nodes 1 and 2 hang behind node 0
+    c["depth"] = dev(np.array([[0, 1, 1]], np.int32))
+    clean = check_attn(c, window)[0]
+    c["v"][0, 1, 0, 5], c["v"][0, 2, 1, 7] = math.inf, -math.inf
+    c["v_cache"][0, 14 - window + 1, 0, 9] = -math.inf                 # seen by node 0 only
+    c["v_cache"][0, 14 - window + 2, 1, 11], c["v"][0, 0, 1, 11] = math.inf, -math.inf          # both seen by all
+    c["v_cache"][0, 13, 0, 3] = math.nan
+    out = ops.tree_attention(**c, window=window).float().view(T, 2, H // 2, D)
+    want = clean.float().view(T, 2, H // 2, D).clone()
+    want[1, 0, :, 5], want[2, 1, :, 7], want[0, 0, :, 9], want[:, 1, :, 11], want[:, 0, :, 3] = math.inf, -math.inf, -math.inf, math.nan, math.nan
+    assert torch.equal(torch.nan_to_num(out, nan=1e9, posinf=2e9, neginf=-2e9), torch.nan_to_num(want, nan=1e9, posinf=2e9, neginf=-2e9))
+
+
+def test_tree_attention_scale():
+    c = attn_case(14, F32, 1, 5, 4, 2, 64, 40, [33])
+    check_attn(c, scale=-0.2)
+    check_attn(c, scale=1.5)
+    d = attn_case(14, BF16, 2, 40, 4, 2, 128, 40, [33])
+    check_attn(d, scale=-0.2)
+    for bad in (0.0, math.inf, math.nan):
+        with pytest.raises((v.VoxError, ValueError), match="scale"):
+            ops.tree_attention(**c, scale=bad)
 
 
 def test_tree_attention_scores_of_minus_infinity_and_nan():

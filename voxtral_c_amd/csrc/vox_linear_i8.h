@@ -152,7 +152,7 @@ template <typename T, int BM, int STAGES> __global__ __launch_bounds__(256) void
     typedef int i32x16 __attribute__((ext_vector_type(16)));
     constexpr int ROWS = BM + I8_BN, STAGE = ROWS * I8_BK, LOADS = ROWS / 32;      // LOADS: instructions per wave and slice
     constexpr int MI = BM / 64, NJ = 2;                                            // 32 x 32 blocks of a wave: rows, channels
-    extern __shared__ __attribute__((aligned(128))) int8_t lds[];
+    extern __shared__ __attribute__((aligned(128))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
     // Each XCD (workgroup number mod 8) works through a range of tiles of its own in which the channels change fastest within bands of an
     // eighth of all channels: its L2 keeps the band's weights, and a row panel is read once per band.
@@ -191,7 +191,7 @@ template <typename T, int BM, int STAGES> __global__ __launch_bounds__(256) void
         if (STAGES == 3 && s + 1 < slices) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (s + STAGES - 1 < slices) issue(s + STAGES - 1);
-        const int8_t *buf = lds + (s % STAGES) * STAGE;
+        const char *buf = lds + (s % STAGES) * STAGE;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             i32x4 wf[NJ], xf[MI];

@@ -136,6 +136,7 @@ int check_attn(const vox_hip_tree_attn_t *a) {
     CHECK(a->kv_heads >= 1 && a->heads >= 1 && a->heads <= 4096 && a->heads % a->kv_heads == 0, "%s: %d heads over %d kv heads", who, a->heads, a->kv_heads);
     CHECK(a->head_dim >= 1 && a->head_dim <= TREE_SCALAR_MAX_D, "%s: head_dim %d (at most %d)", who, a->head_dim, TREE_SCALAR_MAX_D);
     CHECK(a->cap >= 1, "%s: a cache of %d rows", who, a->cap);
+    CHECK(a->scale != 0.f && a->scale - a->scale == 0.f, "%s: scale %g (a finite number other than 0)", who, (double)a->scale);
     CHECK(a->reserved == 0, "%s: reserved is not 0", who);
     return 0;
 }
@@ -155,31 +156,40 @@ bool attn_wide(const vox_hip_tree_attn_t *a) {
         if (r * size >= (int64_t)1 << 31) return false;
     return a->head_dim % unit == 0;
 }
-// Rows (nodes x heads of a kv head) per workgroup: all of them up to 128, so that keys are read once; a wave holds 16 or 32, as many as its
-// registers do.  Splits: enough workgroups for two per CU, but at least one key tile per wave in each.
-struct AttnLaunch { bool wide; int DP, RT, row_waves, row_blocks, splits; int64_t ws; unsigned lds; };
+// Up to 32 rows (nodes x heads of a kv head) the waves of a workgroup have keys of their own, above that rows of their own (64 or 128 per workgroup)
+// and shared keys: see vox_tree_attn.h.  Splits: enough workgroups for two per CU, but at least one key tile per wave in each.
+struct AttnLaunch { bool wide, shared; int DP, RT, row_blocks, key_waves, splits; int64_t ws; };
 AttnLaunch attn_launch(const vox_hip_tree_attn_t *a) {
     AttnLaunch l{};
     l.wide = attn_wide(a);
     if (!l.wide || a->batch == 0 || a->nodes == 0) return l;
     const int64_t R = (int64_t)a->nodes * (a->heads / a->kv_heads);
     l.DP = a->head_dim <= 64 ? 64 : a->head_dim <= 128 ? 128 : 256;
-    l.RT = R <= 16 || l.DP == 256 ? 1 : 2;
-    const int waves = (int)((R + l.RT * 16 - 1) / (l.RT * 16));
-    l.row_waves = waves <= 1 ? 1 : waves <= 2 ? 2 : 4;
-    const int rows = l.RT * 16 * l.row_waves, key_waves = ATTN_WAVES / l.row_waves;
+    l.shared = R > (l.DP == 256 ? 16 : 32);
+    l.RT = l.DP == 256 || R <= 16 || (l.shared && R <= 64) ? 1 : 2;
+    const int rows = l.RT * 16 * (l.shared ? ATTN_WAVES : 1);
+    l.key_waves = l.shared ? 1 : ATTN_WAVES;
     l.row_blocks = (int)((R + rows - 1) / rows);
-    l.lds = (unsigned)(rows * (l.DP + 4) + 2 * key_waves * rows) * 4;
     const int KT = a->dtype == VOX_F32 ? 16 : 32;
     const int64_t keys = a->window > 0 ? std::min(a->cap, a->window) : a->cap, tiles = (keys + KT - 1) / KT + (a->nodes + KT - 1) / KT;
     const int64_t groups = (int64_t)a->batch * a->kv_heads * l.row_blocks;
-    l.splits = (int)std::max<int64_t>(1, std::min<int64_t>({64, 512 / groups, (tiles + key_waves - 1) / key_waves}));
+    l.splits = (int)std::max<int64_t>(1, std::min<int64_t>({64, 512 / groups, (tiles + l.key_waves - 1) / l.key_waves}));
     if (l.splits > 1) l.ws = round_up((int64_t)l.splits * a->batch * a->kv_heads * R * a->head_dim * 4, 256) + (int64_t)l.splits * a->batch * a->kv_heads * R * 8;
     return l;
 }
+template <typename T, int DP, int RT, bool SHARED> void launch_attn2(const TreeAttnArgs &t, const TreeAttnPlan &p, dim3 grid, hipStream_t s) {
+    hipLaunchKernelGGL((k_tree_attn<T, DP, RT, SHARED>), grid, dim3(64 * ATTN_WAVES), (attn_lds<T, DP, RT, SHARED>()), s, t, p);
+}
 template <typename T, int DP> void launch_attn(const TreeAttnArgs &t, const TreeAttnPlan &p, const AttnLaunch &l, dim3 grid, hipStream_t s) {
-    if (l.RT == 1) hipLaunchKernelGGL((k_tree_attn<T, DP, 1>), grid, dim3(64 * ATTN_WAVES), l.lds, s, t, p);
-    else if constexpr (DP < 256) hipLaunchKernelGGL((k_tree_attn<T, DP, 2>), grid, dim3(64 * ATTN_WAVES), l.lds, s, t, p);
+    if constexpr (DP == 256) {
+        if (l.shared) launch_attn2<T, DP, 1, true>(t, p, grid, s);
+        else launch_attn2<T, DP, 1, false>(t, p, grid, s);
+    } else {
+        if (l.shared && l.RT == 2) launch_attn2<T, DP, 2, true>(t, p, grid, s);
+        else if (l.shared) launch_attn2<T, DP, 1, true>(t, p, grid, s);
+        else if (l.RT == 2) launch_attn2<T, DP, 2, false>(t, p, grid, s);
+        else launch_attn2<T, DP, 1, false>(t, p, grid, s);
+    }
 }
 }  // namespace
 extern "C" int64_t vox_hip_tree_attention_workspace(const vox_hip_tree_attn_t *a) {
@@ -207,14 +217,14 @@ extern "C" int vox_hip_tree_attention(const vox_hip_tree_attn_t *a, void *ws, si
         return launched("vox_hip_tree_attention");
     }
     const int R = a->nodes * t.G;
-    TreeAttnPlan p{l.splits, l.row_blocks, l.row_waves, (float *)ws, (float *)((char *)ws + round_up((int64_t)l.splits * a->batch * a->kv_heads * R * a->head_dim * 4, 256))};
+    TreeAttnPlan p{l.splits, l.row_blocks, (float *)ws, (float *)((char *)ws + round_up((int64_t)l.splits * a->batch * a->kv_heads * R * a->head_dim * 4, 256))};
     const dim3 grid((unsigned)(round_up((int64_t)l.splits * a->kv_heads, 8) * l.row_blocks), a->batch);
     by_type(a->dtype, [&](auto z) {
         typedef decltype(z) T;
         if (l.DP == 64) launch_attn<T, 64>(t, p, l, grid, s);
         else if (l.DP == 128) launch_attn<T, 128>(t, p, l, grid, s);
         else launch_attn<T, 256>(t, p, l, grid, s);
-        if (l.splits > 1) hipLaunchKernelGGL(k_tree_attn_join<T>, dim3((R + 3) / 4, a->kv_heads, a->batch), dim3(256), 0, s, t, p);
+        if (l.splits > 1) hipLaunchKernelGGL(k_tree_attn_join<T>, dim3((R + 3) / 4, a->kv_heads, a->batch), dim3(256), 0, s, t, p, l.key_waves);
     });
     return launched("vox_hip_tree_attention");
 }

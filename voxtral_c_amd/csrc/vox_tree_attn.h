@@ -87,16 +87,20 @@ template <typename T> __global__ __launch_bounds__(256) void k_tree_attn_scalar(
 
 
 // ---- matrix-pipe form ----------------------------------------------------------------------------------------------------------
-// The G query heads of a kv head share its keys, so the rows of a (sequence, kv head) are its nodes x G heads, taken in tiles of 16.  A wave
-// owns KT keys at a time and both products are transposed so that nothing passes through LDS:
+// The G query heads of a kv head share its keys, so the rows of a (sequence, kv head) are its nodes x G heads, taken in tiles of 16.  KT keys
+// are a step, and both products are transposed so that the weights never leave their registers:
 //   S^T[key, row] = K . Q^T      K is the A operand (lane: key = lane % 16, its share of the head's dimensions), Q^T stays in registers;
 //   O^T[d, row]  += V^T . P^T    the lane that holds S^T's column (row = lane % 16) for keys 4 c + r, c = lane / 16, holds exactly
-//                                what the B operand wants of P^T if the product's inner index runs over keys in that order, and V is loaded as the
-//                                A operand in the same order: lane m of a 16-lane row takes E = DP / 16 consecutive dimensions of the keys 4 c + r
-//                                and supplies dimension m E + e to the e-th product.
-// Every key and value is loaded once per row block, straight from memory into the registers that the matrix instruction reads, 16 bytes per lane; K of
-// the next tile is requested when the scores are done, V when the outputs are.  Each wave runs its own online softmax (one maximum and sum per
-// row); the waves of a workgroup are joined through LDS at the end, the parts of a long cache by k_tree_attn_join.
+//                                what the B operand wants of P^T if the product's inner index runs over keys in that order, and V is read as the
+//                                A operand in the same order: lane m of a 16-lane row takes VU consecutive dimensions (16 m VU ..) of the keys
+//                                4 c + r and supplies one of them to each of E products.
+// Two ways to the keys:
+//   own      (up to 32 rows) every wave has keys of its own, straight from memory into the registers that the matrix instruction reads, 16 bytes per
+//            lane; K of the next step is requested when the scores are done, V when the outputs are.  Bound by the read of the cache.
+//   shared   (more rows) the four waves have rows of their own and share the steps' keys in LDS, which global_load_lds fills STAGES steps ahead:
+//            nothing of it is in registers, and the cache is read once per 64 or 128 rows.  Bound by the read, or by the products of f32.
+// Each wave runs its own online softmax (one maximum and sum per row); waves with different keys are joined through LDS at the end, the parts of a
+// long cache by k_tree_attn_join.
 template <typename T> struct AttnType;
 template <> struct AttnType<float> {
     static constexpr int KT = 16, SHIFT = 0;
@@ -121,11 +125,9 @@ template <> struct AttnType<f16_t> {
     static constexpr float LAZY = 3.f;
 };
 
-constexpr int ATTN_WAVES = 4;
-// The waves of a workgroup: row_waves of them side by side over the rows (each RT row tiles, the same keys: they share them through L1), the
-// others (key_waves = ATTN_WAVES / row_waves) over the keys.
+constexpr int ATTN_WAVES = 4, ATTN_STAGES = 3;
 struct TreeAttnPlan {
-    int splits, row_blocks, row_waves;
+    int splits, row_blocks;
     float *part_o, *part_ml;      // [splits][batch * Hk][rows][D], [splits][batch * Hk][rows][2]
 };
 
@@ -157,14 +159,13 @@ struct TileRange {
     int64_t first, len;
     int cached, n_cache, n_all, per;
 };
-template <int KT> __device__ __forceinline__ TileRange tile_range(const TreeAttnArgs &a, int b, const TreeAttnPlan &plan) {
+template <int KT> __device__ __forceinline__ TileRange tile_range(const TreeAttnArgs &a, int b, int splits, int key_waves) {
     TileRange r;
     tree_range(a, b, r.first, r.len);
     r.cached = (int)(r.len - r.first);
     r.n_cache = (int)(((int64_t)r.cached + KT - 1) / KT);
     r.n_all = r.n_cache + (a.T + KT - 1) / KT;
-    const int kw = ATTN_WAVES / plan.row_waves;
-    r.per = ((r.n_all + plan.splits - 1) / plan.splits + kw - 1) / kw * kw;
+    r.per = ((r.n_all + splits - 1) / splits + key_waves - 1) / key_waves * key_waves;
     return r;
 }
 
@@ -175,8 +176,16 @@ struct KeyTile {
     int count, wrap, cap;
 };
 
-template <typename T, int DP, int RT> __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_attn(TreeAttnArgs a, TreeAttnPlan plan) {
+// Bytes of LDS of a workgroup: the stages (shared) or Q^T (own, where registers do not hold it), later the outputs; and maxima and sums.
+template <typename T, int DP, int RT, bool SHARED> constexpr int attn_lds() {
+    const int rows = RT * 16 * (SHARED ? ATTN_WAVES : 1), out = rows * (DP + 4) * 4, stages = SHARED ? ATTN_STAGES * 2 * AttnType<T>::KT * DP * (int)sizeof(T) : 0;
+    return (out > stages ? out : stages) + 2 * (SHARED ? 1 : ATTN_WAVES) * rows * 4;
+}
+
+template <typename T, int DP, int RT, bool SHARED>
+__global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_attn(TreeAttnArgs a, TreeAttnPlan plan) {
     typedef AttnType<T> A;
+    typedef typename A::Bits bits_t;
     constexpr int KT = A::KT, E = DP / 16, NK = KT / 16, VK = KT / 4;            // VK: keys per lane of a V operand
     constexpr int U = sizeof(T) == 2 ? 8 : 4;                                    // elements per 16-byte load
     constexpr int KS = DP / (4 * U);                                             // K / Q loads per lane and 16 keys / rows
@@ -184,29 +193,31 @@ template <typename T, int DP, int RT> __global__ __launch_bounds__(64 * ATTN_WAV
     constexpr float LOG2E = 1.44269504088896340736f;
     typedef T kvec __attribute__((ext_vector_type(U)));
     typedef T vvec __attribute__((ext_vector_type(VU)));
-    constexpr int WROWS = RT * 16, LD = DP + 4;                                  // rows of a wave
-    const int RW = plan.row_waves, KW = ATTN_WAVES / RW, ROWS = WROWS * RW;      // rows of a workgroup
-    extern __shared__ __attribute__((aligned(16))) float so[];                   // [ROWS][LD]: Q^T during the loop, then the outputs, one key wave's after another's
-    float *sm = so + ROWS * LD, *sl = sm + KW * ROWS;                            // [KW][ROWS] each
+    constexpr int RW = SHARED ? ATTN_WAVES : 1, KW = ATTN_WAVES / RW;            // waves side by side over rows, over keys
+    constexpr int WROWS = RT * 16, ROWS = WROWS * RW, LD = DP + 4;               // rows of a wave, of the workgroup
+    extern __shared__ __attribute__((aligned(128))) char lds[];
+    float *so = reinterpret_cast<float *>(lds);                                  // [ROWS][LD]: the outputs, one key wave's after another's
+    float *sm = reinterpret_cast<float *>(lds + attn_lds<T, DP, RT, SHARED>()) - 2 * KW * ROWS, *sl = sm + KW * ROWS;        // [KW][ROWS] each
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kw = wave / RW, rw = wave - kw * RW, n16 = lane & 15, c = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, c = lane >> 4;
     // Workgroups that read the same keys (the row blocks of a group) have numbers that differ by 8: they land on one XCD and share its L2.
     const int RB = plan.row_blocks, chunk = blockIdx.x / (8 * RB), in = blockIdx.x - chunk * 8 * RB;
     const int group = chunk * 8 + (in & 7), rb = in >> 3;
     const int b = blockIdx.y, split = group / a.Hk, kvh = group - split * a.Hk;
     if (split >= plan.splits) return;
-    const TileRange tr = tile_range<KT>(a, b, plan);
+    const TileRange tr = tile_range<KT>(a, b, plan.splits, KW);
     const int t_begin = split * tr.per, t_end = min(t_begin + tr.per, tr.n_all);
     if (t_begin >= t_end) return;
-    const int R = a.T * a.G, row0 = rb * ROWS, wrow0 = row0 + rw * WROWS;
+    const int R = a.T * a.G, row0 = rb * ROWS;
+    const int kw = SHARED ? 0 : wave, rw = SHARED ? (wave + split) & (ATTN_WAVES - 1) : 0;       // (idle waves on another SIMD from split to split)
+    const int wrow0 = row0 + rw * WROWS;
     const bool idle = wrow0 >= R;                            // (the last workgroup's waves behind the last row)
 
-    // this lane's query rows
-    int row_depth[RT], row_node[RT];
-    // Q^T as B operands: in registers, or in LDS [RT][KS][64 lanes] where the registers do not hold them (f32, 256 dimensions)
-    constexpr bool QLDS = sizeof(T) == 4 || DP == 256;
+    // this lane's query rows; a negative scale goes into Q's sign
+    constexpr bool QLDS = !SHARED && (sizeof(T) == 4 || DP == 256);
     kvec qf[QLDS ? 1 : RT][QLDS ? 1 : KS];
-    kvec *qs = reinterpret_cast<kvec *>(so) + rw * RT * KS * 64;
+    kvec *qs = reinterpret_cast<kvec *>(lds);                // [RT][KS][64 lanes]
+    int row_depth[RT], row_node[RT];
 #pragma unroll
     for (int t = 0; t < RT; t++) {
         const int row = wrow0 + t * 16 + n16, node = row < R ? row / a.G : 0, h = kvh * a.G + (row - node * a.G);
@@ -218,11 +229,13 @@ template <typename T, int DP, int RT> __global__ __launch_bounds__(64 * ATTN_WAV
             const int d = s * 4 * U + c * U;
             kvec x = kvec(T(0.f));
             if (row < R && d < a.D) x = *reinterpret_cast<const kvec *>(q + d);
+            if (a.scale < 0.f) x = -x;
             if constexpr (!QLDS) qf[t][s] = x;
             else if (kw == 0) qs[(t * KS + s) * 64 + lane] = x;
         }
     }
-    if (QLDS) __syncthreads();
+    const float scale2 = fabsf(a.scale) * LOG2E;
+
     const char *kc = (const char *)((const T *)a.kc + b * a.kc_sb + kvh * a.kc_sh), *vc = (const char *)((const T *)a.vc + b * a.vc_sb + kvh * a.vc_sh);
     const char *kt = (const char *)((const T *)a.k + b * a.k_sb + kvh * a.k_sh), *vt = (const char *)((const T *)a.v + b * a.v_sb + kvh * a.v_sh);
     const int64_t slot_first = tr.first % a.cap;
@@ -268,20 +281,24 @@ template <typename T, int DP, int RT> __global__ __launch_bounds__(64 * ATTN_WAV
         }
         return x.count < 32 ? bits & ((1u << x.count) - 1u) : bits;
     };
-    kvec kf[NK][KS];
+    auto bits_of = [](T x) { return __builtin_bit_cast(bits_t, x); };
+
+    // ---- keys of the wave's own
+    kvec kf[SHARED ? 1 : NK][SHARED ? 1 : KS];
     vvec vf[VK][VL];
     auto load_k = [&](const KeyTile &x) {
+        if constexpr (!SHARED)
 #pragma unroll
-        for (int i = 0; i < NK; i++) {
-            const int key = i * 16 + n16, row = key < x.wrap ? key : key - x.cap;
-            const T *p = reinterpret_cast<const T *>(x.k + (int64_t)row * x.ks);
+            for (int i = 0; i < NK; i++) {
+                const int key = i * 16 + n16, row = key < x.wrap ? key : key - x.cap;
+                const T *p = reinterpret_cast<const T *>(x.k + (int64_t)row * x.ks);
 #pragma unroll
-            for (int s = 0; s < KS; s++) {
-                const int d = s * 4 * U + c * U;
-                if (key < x.count && d < a.D) kf[i][s] = *reinterpret_cast<const kvec *>(p + d);
-                else kf[i][s] = kvec(T(0.f));
+                for (int s = 0; s < KS; s++) {
+                    const int d = s * 4 * U + c * U;
+                    if (key < x.count && d < a.D) kf[i][s] = *reinterpret_cast<const kvec *>(p + d);
+                    else kf[i][s] = kvec(T(0.f));
+                }
             }
-        }
     };
     auto load_v = [&](const KeyTile &x) {
 #pragma unroll
@@ -290,9 +307,27 @@ template <typename T, int DP, int RT> __global__ __launch_bounds__(64 * ATTN_WAV
             const T *p = reinterpret_cast<const T *>(x.v + (int64_t)row * x.vs);
 #pragma unroll
             for (int u = 0; u < VL; u++) {
-                const int d = n16 * E + u * VU;
+                const int d = (u * 16 + n16) * VU;
                 if (key < x.count && d < a.D) vf[j][u] = *reinterpret_cast<const vvec *>(p + d);
                 else vf[j][u] = vvec(T(0.f));
+            }
+        }
+    };
+
+    // ---- keys in LDS: per stage K [KT][DP], V [KT][DP]; 16-byte piece q of row r sits at (q ^ (r & 7)), so that the 8 lanes of one access (8 rows, one
+    // piece each) touch every bank once
+    constexpr int PIECES = DP * (int)sizeof(T) / 16, TILE = KT * DP * (int)sizeof(T), LOADS = TILE / (1024 * ATTN_WAVES);        // LOADS: per wave, for K and for V
+    static_assert(TILE % (1024 * ATTN_WAVES) == 0, "a tile is a whole number of a workgroup's loads");
+    auto piece_at = [](int row, int q) { return (row * PIECES + (q ^ (row & 7))) * 16; };
+    auto issue = [&](int t) {
+        const KeyTile x = tile_at(t);
+        const unsigned base = lds_addr(lds) + (unsigned)((t - t_begin) % ATTN_STAGES) * (2 * TILE);
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int at = (i * ATTN_WAVES + wave) * 64, row = (at + lane) / PIECES, q = ((at + lane) % PIECES) ^ (row & 7), from = row < x.wrap ? row : row - x.cap;
+            if (row < x.count && q * U < a.D) {
+                glds16(x.k + (int64_t)from * x.ks + q * 16, __builtin_amdgcn_readfirstlane(base + at * 16));
+                glds16(x.v + (int64_t)from * x.vs + q * 16, __builtin_amdgcn_readfirstlane(base + TILE + at * 16));
             }
         }
     };
@@ -305,33 +340,90 @@ template <typename T, int DP, int RT> __global__ __launch_bounds__(64 * ATTN_WAV
 #pragma unroll
         for (int e = 0; e < E; e++) o[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const float scale2 = a.scale * LOG2E;
-    typedef typename A::Bits bits_t;
-    auto bits_of = [](T x) { return __builtin_bit_cast(bits_t, x); };
-    bool bad = false;                                        // a masked tile of this wave held a value that is not finite
+    bool bad = false;                                        // a masked tile held a value that is not finite
+    auto v_operand = [&](int e) {
+        kvec av;
+#pragma unroll
+        for (int j = 0; j < VK; j++) av[j] = vf[j][e / VU][e % VU];
+        return av;
+    };
 
-    int t = idle ? t_end : t_begin + kw;
+    int t = SHARED ? t_begin : t_begin + kw;
     KeyTile cur{}, nxt{};
-    if (t < t_end) { cur = tile_at(t); load_k(cur); load_v(cur); }
-    for (; t < t_end; t += KW, cur = nxt) {
+    if constexpr (SHARED) {
+        if (a.D < DP) {                                      // dimensions that no load fills
+            for (int i = tid; i < ATTN_STAGES * 2 * TILE / 16; i += 64 * ATTN_WAVES) reinterpret_cast<uint4 *>(lds)[i] = uint4{0, 0, 0, 0};
+            __syncthreads();
+        }
+#pragma unroll
+        for (int i = 0; i < ATTN_STAGES - 1; i++)
+            if (t + i < t_end) issue(t + i);
+    } else {
+        if (QLDS) __syncthreads();
+        if (t < t_end) { cur = tile_at(t); load_k(cur); load_v(cur); }
+    }
+    for (; t < t_end; t += KW) {
         const bool more = t + KW < t_end;
-        if (more) nxt = tile_at(t + KW);
+        const char *sk = lds, *sv = lds;
+        if constexpr (SHARED) {
+            // Tile t has landed when at most the next tile's loads are in flight; behind the barrier everyone's has, and everyone is done with the
+            // tile that the next loads overwrite (their LDS reads have returned: the compiler may place the products behind the barrier).  A lane
+            // whose piece is not there issues nothing, but its wave does, unless a whole instruction is empty: only then the count is too careful.
+            if (t + 1 < t_end && a.D == DP && t + 1 < tr.n_cache && (int64_t)(t + 2) * KT <= tr.cached) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            cur = tile_at(t);
+            if (t + ATTN_STAGES - 1 < t_end) issue(t + ATTN_STAGES - 1);
+            sk = lds + ((t - t_begin) % ATTN_STAGES) * (2 * TILE);
+            sv = sk + TILE;
+        } else if (more) {
+            nxt = tile_at(t + KW);
+        }
         const bool masked = is_masked(t, cur);
+        if constexpr (SHARED) {
+            // 0 * inf: a value that is not finite must not reach the rows that do not see its key, nor what lies behind the last key.  Such values become
+            // zeros here; what they do to the rows that see them is put in behind the loop.
+            if (masked) {
+                T *v = reinterpret_cast<T *>(const_cast<char *>(sv));
+                for (int i = tid; i < KT * PIECES; i += 64 * ATTN_WAVES) {
+                    const int row = i / PIECES;
+                    kvec x = reinterpret_cast<kvec *>(v)[i];
+                    bool change = row >= cur.count;
+#pragma unroll
+                    for (int j = 0; j < U; j++)
+                        if (row >= cur.count) x[j] = T(0.f);
+                        else if ((bits_of(x[j]) & A::INF) == A::INF) { x[j] = T(0.f); change = true; bad = true; }
+                    if (change) reinterpret_cast<kvec *>(v)[i] = x;
+                }
+                __syncthreads();
+            }
+            if (idle) continue;
+        }
         kvec pf[RT];                                         // the row tiles' weights as the second product's operand
+        f32x4 s[RT][NK];
+        if constexpr (SHARED) {
 #pragma unroll
-        for (int r = 0; r < RT; r++) {
-            f32x4 s[NK];
-#pragma unroll
-            for (int i = 0; i < NK; i++) {
-                s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < NK; i++)
 #pragma unroll
                 for (int x = 0; x < KS; x++) {
-                    kvec q;
-                    if constexpr (QLDS) q = qs[(r * KS + x) * 64 + lane];
-                    else q = qf[r][x];
-                    s[i] = attn_mma<T>(kf[i][x], q, s[i]);
+                    const kvec k = *reinterpret_cast<const kvec *>(sk + piece_at(i * 16 + n16, x * 4 + c));
+#pragma unroll
+                    for (int r = 0; r < RT; r++) s[r][i] = attn_mma<T>(k, qf[r][x], x == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[r][i]);
                 }
-                s[i] *= scale2;
+        }
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            if constexpr (!SHARED) {
+#pragma unroll
+                for (int i = 0; i < NK; i++) {
+                    s[r][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int x = 0; x < KS; x++) {
+                        kvec q;
+                        if constexpr (QLDS) q = qs[(r * KS + x) * 64 + lane];
+                        else q = qf[r][x];
+                        s[r][i] = attn_mma<T>(kf[i][x], q, s[r][i]);
+                    }
+                }
             }
             if (masked) {
                 const unsigned bits = visible(t, cur, r);
@@ -339,15 +431,15 @@ template <typename T, int DP, int RT> __global__ __launch_bounds__(64 * ATTN_WAV
                 for (int i = 0; i < NK; i++)
 #pragma unroll
                     for (int y = 0; y < 4; y++)
-                        if (!((bits >> (i * 16 + c * 4 + y)) & 1u)) s[i][y] = -INFINITY;
+                        if (!((bits >> (i * 16 + c * 4 + y)) & 1u)) s[r][i][y] = -INFINITY;
             }
             // online softmax, base 2; the maximum is only raised when it grows by more than LAZY (weights stay below 2^(LAZY + SHIFT))
-            float mx = s[0][0];
+            float mx = s[r][0][0];
 #pragma unroll
             for (int i = 0; i < NK; i++)
 #pragma unroll
-                for (int y = 0; y < 4; y++) mx = fmaxf(mx, s[i][y]);
-            mx = max_over_c(mx);
+                for (int y = 0; y < 4; y++) mx = fmaxf(mx, s[r][i][y]);
+            mx = max_over_c(mx) * scale2;
             if (__any(mx > m[r] + A::LAZY)) {
                 const float mn = fmaxf(m[r], mx), f = mn == m[r] ? 1.f : __builtin_amdgcn_exp2f(m[r] - mn);
                 l[r] *= f;
@@ -360,26 +452,30 @@ template <typename T, int DP, int RT> __global__ __launch_bounds__(64 * ATTN_WAV
             for (int i = 0; i < NK; i++)
 #pragma unroll
                 for (int y = 0; y < 4; y++) {
-                    s[i][y] = __builtin_amdgcn_exp2f(s[i][y] - base);
-                    l[r] += s[i][y];
-                    pf[r][i * 4 + y] = from_f32<T>(s[i][y]);
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[r][i][y], scale2, -base));
+                    l[r] += p;
+                    pf[r][i * 4 + y] = from_f32<T>(p);
                 }
         }
-        if (more) load_k(nxt);
-        auto v_operand = [&](int e) {
-            kvec av;
+        if constexpr (SHARED) {
 #pragma unroll
-            for (int j = 0; j < VK; j++) av[j] = vf[j][e / VU][e % VU];
-            return av;
-        };
-        if (masked) {
-            // 0 * inf: a value that is not finite must not reach the rows that do not see its key.  It becomes zero here; what it does to the rows
-            // that see it is put in behind the loop.
+            for (int j = 0; j < VK; j++) {
+                const int key = (j >> 2) * 16 + c * 4 + (j & 3);
 #pragma unroll
-            for (int j = 0; j < VK; j++)
+                for (int u = 0; u < VL; u++) {
+                    const int at = (u * 16 + n16) * VU * (int)sizeof(T);         // byte of the row
+                    vf[j][u] = *reinterpret_cast<const vvec *>(sv + piece_at(key, at >> 4) + (at & 15));
+                }
+            }
+        } else {
+            if (more) load_k(nxt);
+            if (masked) {                                    // (as above)
 #pragma unroll
-                for (int e = 0; e < E; e++)
-                    if ((bits_of(vf[j][e / VU][e % VU]) & A::INF) == A::INF) { vf[j][e / VU][e % VU] = T(0.f); bad = true; }
+                for (int j = 0; j < VK; j++)
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+                        if ((bits_of(vf[j][e / VU][e % VU]) & A::INF) == A::INF) { vf[j][e / VU][e % VU] = T(0.f); bad = true; }
+            }
         }
         // O^T += V^T P^T
 #pragma unroll
@@ -388,9 +484,13 @@ template <typename T, int DP, int RT> __global__ __launch_bounds__(64 * ATTN_WAV
 #pragma unroll
             for (int r = 0; r < RT; r++) o[r][e] = attn_mma<T>(av, pf[r], o[r][e]);
         }
-        if (more) load_v(nxt);
+        if constexpr (!SHARED) {
+            if (more) load_v(nxt);
+            cur = nxt;
+        }
     }
-    if (__any(bad)) {
+    if (SHARED) bad = __syncthreads_or(bad);
+    if (__any(bad) && !idle) {
         // Per masked tile and kind (+inf, -inf, NaN): how many such values a row sees is a product of ones; one makes the sum that kind.
         for (t = t_begin + kw; t < t_end; t += KW) {
             cur = tile_at(t);
@@ -432,15 +532,19 @@ template <typename T, int DP, int RT> __global__ __launch_bounds__(64 * ATTN_WAV
         if (c == 0) { sm[kw * ROWS + rw * WROWS + r * 16 + n16] = m[r]; sl[kw * ROWS + rw * WROWS + r * 16 + n16] = l[r]; }
     }
     __syncthreads();
+    if constexpr (KW > 1) {
 #pragma unroll
-    for (int r = 0; r < RT; r++) {
-        const int row = rw * WROWS + r * 16 + n16;
-        float mm = sm[row];
-        for (int w = 1; w < KW; w++) mm = fmaxf(mm, sm[w * ROWS + row]);
-        const float f = m[r] == mm ? 1.f : __builtin_amdgcn_exp2f(m[r] - mm);
+        for (int r = 0; r < RT; r++) {
+            const int row = rw * WROWS + r * 16 + n16;
+            float mm = sm[row];
 #pragma unroll
-        for (int e = 0; e < E; e++) o[r][e] *= f;
+            for (int w = 1; w < KW; w++) mm = fmaxf(mm, sm[w * ROWS + row]);
+            const float f = m[r] == mm ? 1.f : __builtin_amdgcn_exp2f(m[r] - mm);
+#pragma unroll
+            for (int e = 0; e < E; e++) o[r][e] *= f;
+        }
     }
+#pragma unroll
     for (int w = 0; w < KW; w++) {
         if (w == kw) {
 #pragma unroll
@@ -449,7 +553,7 @@ template <typename T, int DP, int RT> __global__ __launch_bounds__(64 * ATTN_WAV
                 for (int y = 0; y < 4; y++)
 #pragma unroll
                     for (int e = 0; e < E; e += 4) {
-                        f32x4 *dst = reinterpret_cast<f32x4 *>(&so[(rw * WROWS + r * 16 + n16) * LD + (c * 4 + y) * E + e]);
+                        f32x4 *dst = reinterpret_cast<f32x4 *>(&so[(rw * WROWS + r * 16 + n16) * LD + ((e / VU) * 16 + c * 4 + y) * VU + e % VU]);
                         const f32x4 x = {o[r][e][y], o[r][e + 1][y], o[r][e + 2][y], o[r][e + 3][y]};
                         *dst = w == 0 ? x : *dst + x;
                     }
@@ -460,7 +564,9 @@ template <typename T, int DP, int RT> __global__ __launch_bounds__(64 * ATTN_WAV
     const int64_t prow = ((int64_t)split * gridDim.y + b) * a.Hk + kvh;
     for (int row = wave; row < ROWS && row0 + row < R; row += ATTN_WAVES) {
         float mm = sm[row], total = 0.f;
+#pragma unroll
         for (int w = 1; w < KW; w++) mm = fmaxf(mm, sm[w * ROWS + row]);
+#pragma unroll
         for (int w = 0; w < KW; w++) total += sl[w * ROWS + row] * (sm[w * ROWS + row] == mm ? 1.f : __builtin_amdgcn_exp2f(sm[w * ROWS + row] - mm));
         const int grow = row0 + row, node = grow / a.G, h = kvh * a.G + (grow - node * a.G);
         if (whole) {
@@ -476,11 +582,11 @@ template <typename T, int DP, int RT> __global__ __launch_bounds__(64 * ATTN_WAV
 }
 
 // Joins the parts of a row: one wave per (row, kv head, sequence); grid (ceil(rows / 4), Hk, batch).
-template <typename T> __global__ __launch_bounds__(256) void k_tree_attn_join(TreeAttnArgs a, TreeAttnPlan plan) {
+template <typename T> __global__ __launch_bounds__(256) void k_tree_attn_join(TreeAttnArgs a, TreeAttnPlan plan, int key_waves) {
     typedef AttnType<T> A;
     const int lane = threadIdx.x & 63, R = a.T * a.G, row = blockIdx.x * 4 + (threadIdx.x >> 6), kvh = blockIdx.y, b = blockIdx.z;
     if (row >= R) return;
-    const TileRange tr = tile_range<A::KT>(a, b, plan);
+    const TileRange tr = tile_range<A::KT>(a, b, plan.splits, key_waves);
     const int n = (tr.n_all + tr.per - 1) / tr.per;
     if (n <= 1) return;                                      // written by its only part
     const int64_t step = (int64_t)gridDim.z * a.Hk * R, at = ((int64_t)b * a.Hk + kvh) * R + row;
