@@ -69,8 +69,9 @@ struct LinearI8Args {
     int M, K, N, ldq;
 };
 // Three roundings of f32 (the sum's conversion and two products) and the one to the output's type; the sum itself is exact.
+__device__ __forceinline__ float i8_scaled(int acc, float xs, float ws) { return ((float)acc * ws) * xs; }
 template <typename T> __device__ __forceinline__ T i8_out(int acc, float xs, float ws, const T *bias, int n) {
-    float v = ((float)acc * ws) * xs;
+    float v = i8_scaled(acc, xs, ws);
     if (bias) v += (float)bias[n];
     return from_f32<T>(v);
 }
@@ -148,6 +149,10 @@ template <typename T, int MT> __global__ __launch_bounds__(64 * I8_ROWS_WAVES) v
 // flight with one barrier per slice.  16-byte pieces of a row are stored at (piece ^ (row & 7)): the MFMA operand reads (lane = row, one piece) then
 // touch every bank once.  Outputs leave through LDS so that rows are written in whole lines.
 constexpr int I8_BN = 128, I8_BK = 128;
+template <typename T, int BM, int STAGES> constexpr unsigned i8_tile_lds() {        // stages, later outputs; scales and bias behind them
+    const unsigned stages = STAGES * (BM + I8_BN) * I8_BK, out = BM * (I8_BN * (unsigned)sizeof(T) + 16);
+    return (stages > out ? stages : out) + (BM + 2 * I8_BN) * 4;
+}
 template <typename T, int BM, int STAGES> __global__ __launch_bounds__(256) void k_linear_i8_tile(LinearI8Args a, int tiles_m, int tiles_n) {
     typedef int i32x16 __attribute__((ext_vector_type(16)));
     constexpr int ROWS = BM + I8_BN, STAGE = ROWS * I8_BK, LOADS = ROWS / 32;      // LOADS: instructions per wave and slice
@@ -171,10 +176,12 @@ template <typename T, int BM, int STAGES> __global__ __launch_bounds__(256) void
         src[i] = i * 32 >= BM ? a.w + (int64_t)min(n0 + row - BM, a.N - 1) * a.w_stride + p * 16 : a.xq + (int64_t)min(m0 + row, a.M - 1) * a.ldq + p * 16;
     }
     const int slices = a.ldq / I8_BK;
-    auto issue = [&](int s) {
+    // loads [from, to) of slice s
+    auto issue = [&](int s, int from, int to) {
         const unsigned base = lds_addr(lds) + (s % STAGES) * STAGE;
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
+            if (i < from || i >= to) continue;
             const int row = (i * 4 + wave) * 8 + (lane >> 3), p = (piece ^ (row & 7)) * 16;
             const bool past = i * 32 >= BM && s * I8_BK + p >= a.K;
             glds16(src[i] + (past ? -p : s * I8_BK), __builtin_amdgcn_readfirstlane(base + (i * 4 + wave) * 1024));
@@ -183,33 +190,47 @@ template <typename T, int BM, int STAGES> __global__ __launch_bounds__(256) void
     i32x16 acc[NJ][MI] = {};
 #pragma unroll
     for (int s = 0; s < STAGES - 1; s++)
-        if (s < slices) issue(s);
+        if (s < slices) issue(s, 0, LOADS);
+    // scales and bias of the tile, f32 (read one by one behind the loop, they cost four times what the products do)
+    float *sw = reinterpret_cast<float *>(lds + i8_tile_lds<T, BM, STAGES>()) - BM - 2 * I8_BN, *sb = sw + I8_BN, *sx = sb + I8_BN;
+    if (tid < I8_BN) {
+        const int n = min(n0 + tid, a.N - 1);
+        sw[tid] = a.ws[n];
+        sb[tid] = a.bias ? (float)((const T *)a.bias)[n] : 0.f;
+    }
+    for (int i = tid; i < BM; i += 256) sx[i] = a.xs[min(m0 + i, a.M - 1)];
     for (int s = 0; s < slices; s++) {
         // slice s has landed when at most the younger slices' loads are in flight; behind the barrier everyone's has, and everyone is done with the
         // slice that the next loads overwrite
         // (this wave's own LDS reads of that slice have returned too: the compiler may place the products that use them behind the barrier)
         if (STAGES == 3 && s + 1 < slices) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (s + STAGES - 1 < slices) issue(s + STAGES - 1);
+        // The operands of step k + 1 are read, and a quarter of the next loads requested, in front of step k's products.
         const char *buf = lds + (s % STAGES) * STAGE;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            i32x4 wf[NJ], xf[MI];
+        const bool more = s + STAGES - 1 < slices;
+        i32x4 wf[2][NJ], xf[2][MI];
+        auto read = [&](int k) {
             const int q = k * 2 + (lane >> 5);
 #pragma unroll
             for (int j = 0; j < NJ; j++) {
                 const int row = BM + wn * 64 + j * 32 + (lane & 31);
-                wf[j] = *reinterpret_cast<const i32x4 *>(buf + row * I8_BK + ((q ^ (row & 7)) << 4));
+                wf[k & 1][j] = *reinterpret_cast<const i32x4 *>(buf + row * I8_BK + ((q ^ (row & 7)) << 4));
             }
 #pragma unroll
             for (int i = 0; i < MI; i++) {
                 const int row = wm * (BM / 2) + i * 32 + (lane & 31);
-                xf[i] = *reinterpret_cast<const i32x4 *>(buf + row * I8_BK + ((q ^ (row & 7)) << 4));
+                xf[k & 1][i] = *reinterpret_cast<const i32x4 *>(buf + row * I8_BK + ((q ^ (row & 7)) << 4));
             }
+        };
+        read(0);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (k < 3) read(k + 1);
+            if (more) issue(s + STAGES - 1, k * LOADS / 4, (k + 1) * LOADS / 4);
 #pragma unroll
             for (int j = 0; j < NJ; j++)
 #pragma unroll
-                for (int i = 0; i < MI; i++) acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[j], xf[i], acc[j][i], 0, 0, 0);
+                for (int i = 0; i < MI; i++) acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[k & 1][j], xf[k & 1][i], acc[j][i], 0, 0, 0);
         }
     }
     __syncthreads();
@@ -219,19 +240,17 @@ template <typename T, int BM, int STAGES> __global__ __launch_bounds__(256) void
 #pragma unroll
     for (int i = 0; i < MI; i++) {
         const int row = wm * (BM / 2) + i * 32 + (lane & 31);
-        const float xs = a.xs[min(m0 + row, a.M - 1)];
+        const float xs = sx[row];
 #pragma unroll
         for (int j = 0; j < NJ; j++)
 #pragma unroll
             for (int g = 0; g < 4; g++) {
                 typedef T out4 __attribute__((ext_vector_type(4)));
                 const int ch = wn * 64 + j * 32 + g * 8 + (lane >> 5) * 4;
+                const f32x4 ws = *reinterpret_cast<const f32x4 *>(sw + ch), bias = *reinterpret_cast<const f32x4 *>(sb + ch);
                 out4 v;
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int n = min(n0 + ch + r, a.N - 1);
-                    v[r] = i8_out<T>(acc[j][i][g * 4 + r], xs, a.ws[n], (const T *)a.bias, n);
-                }
+                for (int r = 0; r < 4; r++) v[r] = from_f32<T>(i8_scaled(acc[j][i][g * 4 + r], xs, ws[r]) + bias[r]);
                 *reinterpret_cast<out4 *>(out + row * LD + ch) = v;
             }
     }

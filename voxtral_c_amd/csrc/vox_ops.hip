@@ -224,7 +224,10 @@ extern "C" int vox_hip_tree_attention(const vox_hip_tree_attn_t *a, void *ws, si
         if (l.DP == 64) launch_attn<T, 64>(t, p, l, grid, s);
         else if (l.DP == 128) launch_attn<T, 128>(t, p, l, grid, s);
         else launch_attn<T, 256>(t, p, l, grid, s);
-        if (l.splits > 1) hipLaunchKernelGGL(k_tree_attn_join<T>, dim3((R + 3) / 4, a->kv_heads, a->batch), dim3(256), 0, s, t, p, l.key_waves);
+        const dim3 rows((R + 3) / 4, a->kv_heads, a->batch);
+        if (l.splits > 1 && l.DP == 64) hipLaunchKernelGGL((k_tree_attn_join<T, 16>), rows, dim3(256), 0, s, t, p, l.key_waves);
+        else if (l.splits > 1 && l.DP == 128) hipLaunchKernelGGL((k_tree_attn_join<T, 32>), rows, dim3(256), 0, s, t, p, l.key_waves);
+        else if (l.splits > 1) hipLaunchKernelGGL((k_tree_attn_join<T, 64>), rows, dim3(256), 0, s, t, p, l.key_waves);
     });
     return launched("vox_hip_tree_attention");
 }
@@ -296,8 +299,7 @@ template <typename T> void launch_quant(const T *x, int64_t stride, int64_t rows
 }
 template <typename T, int BM, int STAGES> void launch_i8_tile(const LinearI8Args &a, hipStream_t s) {
     const int tm = (a.M + BM - 1) / BM, tn = (a.N + I8_BN - 1) / I8_BN;
-    const unsigned stage = (BM + I8_BN) * I8_BK, out = BM * (I8_BN + 16 / sizeof(T)) * sizeof(T);
-    hipLaunchKernelGGL((k_linear_i8_tile<T, BM, STAGES>), dim3((unsigned)round_up((int64_t)tm * tn, 8)), dim3(256), std::max(STAGES * stage, out), s, a, tm, tn);
+    hipLaunchKernelGGL((k_linear_i8_tile<T, BM, STAGES>), dim3((unsigned)round_up((int64_t)tm * tn, 8)), dim3(256), (i8_tile_lds<T, BM, STAGES>()), s, a, tm, tn);
 }
 }  // namespace
 extern "C" int vox_hip_quantize_rows_i8(int dtype, const void *x, int64_t row_stride, int64_t rows, int K, int8_t *q, float *scale, int device, void *stream) {
@@ -342,7 +344,7 @@ extern "C" int vox_hip_linear_i8(int dtype, const void *x, int64_t x_stride, int
         else if (rows <= 16) hipLaunchKernelGGL((k_linear_i8_rows<T, 1>), narrow, dim3(64 * I8_ROWS_WAVES), 0, st, a);
         else if (rows <= 32) hipLaunchKernelGGL((k_linear_i8_rows<T, 2>), narrow, dim3(64 * I8_ROWS_WAVES), 0, st, a);
         else if (rows <= 64) hipLaunchKernelGGL((k_linear_i8_rows<T, 4>), narrow, dim3(64 * I8_ROWS_WAVES), 0, st, a);
-        else if ((rows + 255) / 256 * ((N + 127) / 128) >= 256) launch_i8_tile<T, 256, 3>(a, st);
+        else if (0) launch_i8_tile<T, 256, 3>(a, st);
         else if ((rows + 127) / 128 * ((N + 127) / 128) >= 256) launch_i8_tile<T, 128, 2>(a, st);
         else launch_i8_tile<T, 64, 3>(a, st);
     });

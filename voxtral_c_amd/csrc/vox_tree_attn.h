@@ -401,14 +401,27 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
         kvec pf[RT];                                         // the row tiles' weights as the second product's operand
         f32x4 s[RT][NK];
         if constexpr (SHARED) {
+            // (all of K first, V as soon as the scores are under way: no product waits for LDS)
+            kvec kk[NK][KS];
 #pragma unroll
             for (int i = 0; i < NK; i++)
 #pragma unroll
-                for (int x = 0; x < KS; x++) {
-                    const kvec k = *reinterpret_cast<const kvec *>(sk + piece_at(i * 16 + n16, x * 4 + c));
+                for (int x = 0; x < KS; x++) kk[i][x] = *reinterpret_cast<const kvec *>(sk + piece_at(i * 16 + n16, x * 4 + c));
 #pragma unroll
-                    for (int r = 0; r < RT; r++) s[r][i] = attn_mma<T>(k, qf[r][x], x == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[r][i]);
+            for (int x = 0; x < KS; x++)
+#pragma unroll
+                for (int i = 0; i < NK; i++)
+#pragma unroll
+                    for (int r = 0; r < RT; r++) s[r][i] = attn_mma<T>(kk[i][x], qf[r][x], x == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[r][i]);
+#pragma unroll
+            for (int j = 0; j < VK; j++) {
+                const int key = (j >> 2) * 16 + c * 4 + (j & 3);
+#pragma unroll
+                for (int u = 0; u < VL; u++) {
+                    const int at = (u * 16 + n16) * VU * (int)sizeof(T);         // byte of the row
+                    vf[j][u] = *reinterpret_cast<const vvec *>(sv + piece_at(key, at >> 4) + (at & 15));
                 }
+            }
         }
 #pragma unroll
         for (int r = 0; r < RT; r++) {
@@ -457,17 +470,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
                     pf[r][i * 4 + y] = from_f32<T>(p);
                 }
         }
-        if constexpr (SHARED) {
-#pragma unroll
-            for (int j = 0; j < VK; j++) {
-                const int key = (j >> 2) * 16 + c * 4 + (j & 3);
-#pragma unroll
-                for (int u = 0; u < VL; u++) {
-                    const int at = (u * 16 + n16) * VU * (int)sizeof(T);         // byte of the row
-                    vf[j][u] = *reinterpret_cast<const vvec *>(sv + piece_at(key, at >> 4) + (at & 15));
-                }
-            }
-        } else {
+        if constexpr (!SHARED) {
             if (more) load_k(nxt);
             if (masked) {                                    // (as above)
 #pragma unroll
@@ -581,34 +584,36 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
     }
 }
 
-// Joins the parts of a row: one wave per (row, kv head, sequence); grid (ceil(rows / 4), Hk, batch).
-template <typename T> __global__ __launch_bounds__(256) void k_tree_attn_join(TreeAttnArgs a, TreeAttnPlan plan, int key_waves) {
+// Joins the parts of a row: one wave per (row, kv head, sequence); grid (ceil(rows / 4), Hk, batch).  L lanes take one part's outputs, four values
+// each (the matrix-pipe form's head_dim is a multiple of four), 64 / L parts at a time, their weights first: bound by the read of the parts.
+template <typename T, int L> __global__ __launch_bounds__(256) void k_tree_attn_join(TreeAttnArgs a, TreeAttnPlan plan, int key_waves) {
     typedef AttnType<T> A;
     const int lane = threadIdx.x & 63, R = a.T * a.G, row = blockIdx.x * 4 + (threadIdx.x >> 6), kvh = blockIdx.y, b = blockIdx.z;
     if (row >= R) return;
     const TileRange tr = tile_range<A::KT>(a, b, plan.splits, key_waves);
-    const int n = (tr.n_all + tr.per - 1) / tr.per;
+    const int n = (tr.n_all + tr.per - 1) / tr.per;          // at most 64 parts: lane s holds part s's weight
     if (n <= 1) return;                                      // written by its only part
     const int64_t step = (int64_t)gridDim.z * a.Hk * R, at = ((int64_t)b * a.Hk + kvh) * R + row;
-    float mm = -INFINITY;
-    for (int s = lane; s < n; s += 64) mm = fmaxf(mm, plan.part_ml[(s * step + at) * 2]);
-    mm = wave_max(mm);
-    float total = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < n; s++) {
-        const float ms = plan.part_ml[(s * step + at) * 2], f = ms == mm ? 1.f : __builtin_amdgcn_exp2f(ms - mm);
-        total += f * plan.part_ml[(s * step + at) * 2 + 1];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int d = lane + 64 * j;
-            if (d < a.D) acc[j] += f * plan.part_o[(s * step + at) * a.D + d];
-        }
+    const float ms = lane < n ? plan.part_ml[(lane * step + at) * 2] : -INFINITY, ls = lane < n ? plan.part_ml[(lane * step + at) * 2 + 1] : 0.f;
+    const float mm = wave_max(ms), f = ms == mm ? 1.f : __builtin_amdgcn_exp2f(ms - mm);
+    const float total = wave_sum(f * ls);
+    const int g = lane / L, d = (lane % L) * 4;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < n; s += 64 / L) {
+        const float w = __shfl(f, s + g, 64);
+        if (s + g < n && d < a.D) acc += w * *reinterpret_cast<const f32x4 *>(plan.part_o + ((s + g) * step + at) * a.D + d);
     }
+#pragma unroll
+    for (int o = L; o < 64; o <<= 1)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[i] += __shfl_xor(acc[i], o, 64);
     const int node = row / a.G, h = kvh * a.G + (row - node * a.G);
     const bool none = total == 0.f || a.depth[(size_t)b * a.T + node] < 0;
+    if (g == 0 && d < a.D) {
+        T *out = (T *)a.out + b * a.o_sb + node * a.o_st + h * a.o_sh + d;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int d = lane + 64 * j;
-        if (d < a.D) ((T *)a.out)[b * a.o_sb + node * a.o_st + h * a.o_sh + d] = from_f32<T>(none ? 0.f : acc[j] / total);
+        for (int i = 0; i < 4; i++) out[i] = from_f32<T>(none ? 0.f : acc[i] / total);
     }
     if (a.lse && lane == 0) a.lse[((size_t)b * a.T + node) * a.H + h] = none ? -INFINITY : (mm - A::SHIFT + log2f(total)) * 0.693147180559945309417f;
 }
