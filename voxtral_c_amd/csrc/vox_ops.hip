@@ -141,8 +141,8 @@ int check_attn(const vox_hip_tree_attn_t *a) {
     return 0;
 }
 
-// The matrix-pipe kernel takes 16-byte loads: every row of every operand starts on 16 bytes and holds whole loads, and rows of a cache
-// lie less than 2^31 bytes apart.  Everything else runs on the scalar kernel.
+// The matrix-pipe kernel takes 16-byte loads: every row of every operand starts on 16 bytes and holds whole loads, and keys lie less than 2^26
+// bytes apart (offsets within a tile are 32 bits).  Everything else runs on the scalar kernel.
 bool attn_wide(const vox_hip_tree_attn_t *a) {
     const int size = dtype_size(a->dtype), unit = 16 / size;
     const void *p[5] = {a->q, a->k, a->v, a->k_cache, a->v_cache};
@@ -153,7 +153,7 @@ bool attn_wide(const vox_hip_tree_attn_t *a) {
         if (st[i] % unit) return false;
     const int64_t rows[4] = {a->k_st, a->v_st, a->kc_ss, a->vc_ss};
     for (int64_t r : rows)
-        if (r * size >= (int64_t)1 << 31) return false;
+        if (r * size >= (int64_t)1 << 26) return false;
     return a->head_dim % unit == 0;
 }
 // Up to 32 rows (nodes x heads of a kv head) the waves of a workgroup have keys of their own, above that rows of their own (64 or 128 per workgroup)

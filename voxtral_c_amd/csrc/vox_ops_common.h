@@ -20,6 +20,13 @@ template <typename T, int N> __device__ __forceinline__ void load_vec(float (&o)
     for (int i = 0; i < N; i++) o[i] = (float)v[i];
 }
 
+// glds16 (vox_common.h) from a wave-uniform address and a 32-bit offset per lane.
+__device__ __forceinline__ void glds16_at(const void *base, unsigned offset, unsigned lds_base) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(offset), "s"(base), "s"(lds_base) : "memory");
+}
+
 __device__ __forceinline__ int wave_sum_i(int v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);

@@ -237,57 +237,71 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
     const float scale2 = fabsf(a.scale) * LOG2E;
 
     const char *kc = (const char *)((const T *)a.kc + b * a.kc_sb + kvh * a.kc_sh), *vc = (const char *)((const T *)a.vc + b * a.vc_sb + kvh * a.vc_sh);
-    const char *kt = (const char *)((const T *)a.k + b * a.k_sb + kvh * a.k_sh), *vt = (const char *)((const T *)a.v + b * a.v_sb + kvh * a.v_sh);
-    const int64_t slot_first = tr.first % a.cap;
+    const int ks = (int)a.kc_ss * (int)sizeof(T), vs = (int)a.vc_ss * (int)sizeof(T);            // (less than 2^26: attn_wide)
+    const unsigned slot_first = (unsigned)(tr.first % a.cap);
+    auto slot_of = [&](int t) {
+        const unsigned slot = slot_first + (unsigned)t * KT;
+        return slot >= (unsigned)a.cap ? slot - a.cap : slot;
+    };
+    // Tiles [full_begin, full_end) are seen whole by every row: behind the window's edge of the deepest node, in front of the cache's end.  A tile of
+    // those that the ring does not break is plain: its rows follow each other, and a lane's offsets within it are the same for every tile.
+    const int edge = (int)max(tr.len + 1 - a.window - tr.first, (int64_t)-(1 << 30));            // first position of a window at depth 0, from `first`
+    const int full_begin = a.window > 0 && edge + a.T > 0 ? (edge + a.T - 1) / KT + 1 : 0, full_end = tr.cached / KT;
+    auto is_masked = [&](int t) { return t < full_begin || t >= full_end; };
+    auto is_plain = [&](int t) { return a.D == DP && t < full_end && slot_of(t) + KT <= (unsigned)a.cap; };
     auto tile_at = [&](int t) {
         KeyTile x;
         if (t < tr.n_cache) {
-            const int off = t * KT;
-            int64_t slot = slot_first + off;
-            if (slot >= a.cap) slot -= a.cap;
-            x.k = kc + slot * a.kc_ss * (int)sizeof(T);
-            x.v = vc + slot * a.vc_ss * (int)sizeof(T);
-            x.ks = (int)(a.kc_ss * (int)sizeof(T));
-            x.vs = (int)(a.vc_ss * (int)sizeof(T));
-            x.count = min(KT, tr.cached - off);
+            const int64_t slot = slot_of(t);
+            x.k = kc + slot * ks;
+            x.v = vc + slot * vs;
+            x.ks = ks;
+            x.vs = vs;
+            x.count = min(KT, tr.cached - t * KT);
             x.wrap = (int)min((int64_t)KT, a.cap - slot);
         } else {
             const int off = (t - tr.n_cache) * KT;
-            x.k = kt + off * a.k_st * (int)sizeof(T);
-            x.v = vt + off * a.v_st * (int)sizeof(T);
-            x.ks = (int)(a.k_st * (int)sizeof(T));
-            x.vs = (int)(a.v_st * (int)sizeof(T));
+            x.k = (const char *)((const T *)a.k + b * a.k_sb + kvh * a.k_sh + off * a.k_st);
+            x.v = (const char *)((const T *)a.v + b * a.v_sb + kvh * a.v_sh + off * a.v_st);
+            x.ks = (int)a.k_st * (int)sizeof(T);
+            x.vs = (int)a.v_st * (int)sizeof(T);
             x.count = min(KT, a.T - off);
             x.wrap = KT;
         }
         x.cap = a.cap;
         return x;
     };
-    // Does every row see the whole tile?  And which of its keys (bit i) does row tile r's row of this lane see?
-    auto is_masked = [&](int t, const KeyTile &x) {
-        return t >= tr.n_cache || x.count < KT || (a.window > 0 && tr.first + (int64_t)t * KT <= tr.len + a.T - a.window);
-    };
-    auto visible = [&](int t, const KeyTile &x, int r) {
+    // Which of a tile's keys (bit i) does row tile r's row of this lane see?
+    auto visible = [&](int t, int count, int r) {
         unsigned bits = 0xffffffffu;
         if (t >= tr.n_cache) {
             const int off = (t - tr.n_cache) * KT;
             bits = (unsigned)(a.ancestors[((size_t)b * a.T + row_node[r]) * a.W + (off >> 6)] >> (off & 63));
             if (a.window > 0)
-                for (int j = 0; j < x.count; j++)
+                for (int j = 0; j < count; j++)
                     if (a.depth[(size_t)b * a.T + off + j] <= row_depth[r] - a.window) bits &= ~(1u << j);
         } else if (a.window > 0) {
-            const int64_t below = tr.len + row_depth[r] - a.window - (tr.first + (int64_t)t * KT) + 1;       // keys in front of the row's window
-            bits = below >= 32 ? 0u : below <= 0 ? 0xffffffffu : 0xffffffffu << (int)below;
+            const int below = edge + row_depth[r] - t * KT;  // keys in front of the row's window
+            bits = below >= 32 ? 0u : below <= 0 ? 0xffffffffu : 0xffffffffu << below;
         }
-        return x.count < 32 ? bits & ((1u << x.count) - 1u) : bits;
+        return count < 32 ? bits & ((1u << count) - 1u) : bits;
     };
     auto bits_of = [](T x) { return __builtin_bit_cast(bits_t, x); };
 
     // ---- keys of the wave's own
     kvec kf[SHARED ? 1 : NK][SHARED ? 1 : KS];
     vvec vf[VK][VL];
-    auto load_k = [&](const KeyTile &x) {
-        if constexpr (!SHARED)
+    auto load_k = [&](int t) {
+        if constexpr (!SHARED) {
+            if (is_plain(t)) {
+                const char *base = kc + (int64_t)slot_of(t) * ks;
+#pragma unroll
+                for (int i = 0; i < NK; i++)
+#pragma unroll
+                    for (int s = 0; s < KS; s++) kf[i][s] = *reinterpret_cast<const kvec *>(base + ((unsigned)((i * 16 + n16) * ks + c * 16) + s * 64));
+                return;
+            }
+            const KeyTile x = tile_at(t);
 #pragma unroll
             for (int i = 0; i < NK; i++) {
                 const int key = i * 16 + n16, row = key < x.wrap ? key : key - x.cap;
@@ -299,8 +313,19 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
                     else kf[i][s] = kvec(T(0.f));
                 }
             }
+        }
     };
-    auto load_v = [&](const KeyTile &x) {
+    auto load_v = [&](int t) {
+        if (!SHARED && is_plain(t)) {
+            const char *base = vc + (int64_t)slot_of(t) * vs;
+#pragma unroll
+            for (int j = 0; j < VK; j++)
+#pragma unroll
+                for (int u = 0; u < VL; u++)
+                    vf[j][u] = *reinterpret_cast<const vvec *>(base + ((unsigned)(((j >> 2) * 16 + c * 4 + (j & 3)) * vs + n16 * VU * (int)sizeof(T)) + u * 16 * VU * (int)sizeof(T)));
+            return;
+        }
+        const KeyTile x = tile_at(t);
 #pragma unroll
         for (int j = 0; j < VK; j++) {
             const int key = (j >> 2) * 16 + c * 4 + (j & 3), row = key < x.wrap ? key : key - x.cap;
@@ -319,9 +344,19 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
     constexpr int PIECES = DP * (int)sizeof(T) / 16, TILE = KT * DP * (int)sizeof(T), LOADS = TILE / (1024 * ATTN_WAVES);        // LOADS: per wave, for K and for V
     static_assert(TILE % (1024 * ATTN_WAVES) == 0, "a tile is a whole number of a workgroup's loads");
     auto piece_at = [](int row, int q) { return (row * PIECES + (q ^ (row & 7))) * 16; };
-    auto issue = [&](int t) {
+    auto issue = [&](int t, int stage) {
+        const unsigned base = lds_addr(lds) + (unsigned)stage * (2 * TILE);
+        if (is_plain(t)) {
+            const char *k = kc + (int64_t)slot_of(t) * ks, *v = vc + (int64_t)slot_of(t) * vs;
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) {
+                const int at = (i * ATTN_WAVES + wave) * 64, row = (at + lane) / PIECES, q = ((at + lane) % PIECES) ^ (row & 7);
+                glds16_at(k, (unsigned)(row * ks + q * 16), __builtin_amdgcn_readfirstlane(base + at * 16));
+                glds16_at(v, (unsigned)(row * vs + q * 16), __builtin_amdgcn_readfirstlane(base + TILE + at * 16));
+            }
+            return;
+        }
         const KeyTile x = tile_at(t);
-        const unsigned base = lds_addr(lds) + (unsigned)((t - t_begin) % ATTN_STAGES) * (2 * TILE);
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
             const int at = (i * ATTN_WAVES + wave) * 64, row = (at + lane) / PIECES, q = ((at + lane) % PIECES) ^ (row & 7), from = row < x.wrap ? row : row - x.cap;
@@ -348,8 +383,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
         return av;
     };
 
-    int t = SHARED ? t_begin : t_begin + kw;
-    KeyTile cur{}, nxt{};
+    int t = SHARED ? t_begin : t_begin + kw, stage = 0;
     if constexpr (SHARED) {
         if (a.D < DP) {                                      // dimensions that no load fills
             for (int i = tid; i < ATTN_STAGES * 2 * TILE / 16; i += 64 * ATTN_WAVES) reinterpret_cast<uint4 *>(lds)[i] = uint4{0, 0, 0, 0};
@@ -357,40 +391,38 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
         }
 #pragma unroll
         for (int i = 0; i < ATTN_STAGES - 1; i++)
-            if (t + i < t_end) issue(t + i);
+            if (t + i < t_end) issue(t + i, i);
     } else {
         if (QLDS) __syncthreads();
-        if (t < t_end) { cur = tile_at(t); load_k(cur); load_v(cur); }
+        if (t < t_end) { load_k(t); load_v(t); }
     }
     for (; t < t_end; t += KW) {
-        const bool more = t + KW < t_end;
+        const bool more = t + KW < t_end, masked = is_masked(t);
         const char *sk = lds, *sv = lds;
         if constexpr (SHARED) {
             // Tile t has landed when at most the next tile's loads are in flight; behind the barrier everyone's has, and everyone is done with the
-            // tile that the next loads overwrite (their LDS reads have returned: the compiler may place the products behind the barrier).  A lane
-            // whose piece is not there issues nothing, but its wave does, unless a whole instruction is empty: only then the count is too careful.
-            if (t + 1 < t_end && a.D == DP && t + 1 < tr.n_cache && (int64_t)(t + 2) * KT <= tr.cached) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
+            // tile that the next loads overwrite (their LDS reads have returned: the compiler may place the products behind the barrier).  Only of a
+            // whole tile it is certain that every wave has issued all its loads.
+            if (more && a.D == DP && t + 1 < full_end) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            cur = tile_at(t);
-            if (t + ATTN_STAGES - 1 < t_end) issue(t + ATTN_STAGES - 1);
-            sk = lds + ((t - t_begin) % ATTN_STAGES) * (2 * TILE);
+            if (t + ATTN_STAGES - 1 < t_end) issue(t + ATTN_STAGES - 1, stage == 0 ? ATTN_STAGES - 1 : stage - 1);
+            sk = lds + stage * (2 * TILE);
             sv = sk + TILE;
-        } else if (more) {
-            nxt = tile_at(t + KW);
+            stage = stage == ATTN_STAGES - 1 ? 0 : stage + 1;
         }
-        const bool masked = is_masked(t, cur);
         if constexpr (SHARED) {
             // 0 * inf: a value that is not finite must not reach the rows that do not see its key, nor what lies behind the last key.  Such values become
             // zeros here; what they do to the rows that see them is put in behind the loop.
             if (masked) {
+                const int count = tile_at(t).count;
                 T *v = reinterpret_cast<T *>(const_cast<char *>(sv));
                 for (int i = tid; i < KT * PIECES; i += 64 * ATTN_WAVES) {
                     const int row = i / PIECES;
                     kvec x = reinterpret_cast<kvec *>(v)[i];
-                    bool change = row >= cur.count;
+                    bool change = row >= count;
 #pragma unroll
                     for (int j = 0; j < U; j++)
-                        if (row >= cur.count) x[j] = T(0.f);
+                        if (row >= count) x[j] = T(0.f);
                         else if ((bits_of(x[j]) & A::INF) == A::INF) { x[j] = T(0.f); change = true; bad = true; }
                     if (change) reinterpret_cast<kvec *>(v)[i] = x;
                 }
@@ -439,7 +471,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
                 }
             }
             if (masked) {
-                const unsigned bits = visible(t, cur, r);
+                const unsigned bits = visible(t, tile_at(t).count, r);
 #pragma unroll
                 for (int i = 0; i < NK; i++)
 #pragma unroll
@@ -471,7 +503,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
                 }
         }
         if constexpr (!SHARED) {
-            if (more) load_k(nxt);
+            if (more) load_k(t + KW);
             if (masked) {                                    // (as above)
 #pragma unroll
                 for (int j = 0; j < VK; j++)
@@ -488,24 +520,22 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
             for (int r = 0; r < RT; r++) o[r][e] = attn_mma<T>(av, pf[r], o[r][e]);
         }
         if constexpr (!SHARED) {
-            if (more) load_v(nxt);
-            cur = nxt;
+            if (more) load_v(t + KW);
         }
     }
     if (SHARED) bad = __syncthreads_or(bad);
     if (__any(bad) && !idle) {
         // Per masked tile and kind (+inf, -inf, NaN): how many such values a row sees is a product of ones; one makes the sum that kind.
         for (t = t_begin + kw; t < t_end; t += KW) {
-            cur = tile_at(t);
-            if (!is_masked(t, cur)) continue;
-            load_v(cur);
+            if (!is_masked(t)) continue;
+            load_v(t);
 #pragma unroll 1
             for (int kind = 0; kind < 3; kind++) {
                 const float value = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN;
                 const bits_t inf = kind == 0 ? A::INF : (bits_t)(A::INF | A::SIGN);
 #pragma unroll
                 for (int r = 0; r < RT; r++) {
-                    const unsigned sees = visible(t, cur, r);
+                    const unsigned sees = visible(t, tile_at(t).count, r);
                     kvec one;
 #pragma unroll
                     for (int j = 0; j < VK; j++) one[j] = (sees >> ((j >> 2) * 16 + c * 4 + (j & 3))) & 1u ? T(1.f) : T(0.f);
