@@ -156,7 +156,7 @@ bool attn_wide(const vox_hip_tree_attn_t *a) {
         if (r * size >= (int64_t)1 << 26) return false;
     return a->head_dim % unit == 0;
 }
-// Up to 32 rows (nodes x heads of a kv head) the waves of a workgroup have keys of their own, above that rows of their own (64 or 128 per workgroup)
+// Up to 16 rows (nodes x heads of a kv head; 32 where a head has up to 64 dimensions) the waves of a workgroup have keys of their own, above that rows of their own (64 or 128 per workgroup)
 // and shared keys: see vox_tree_attn.h.  Splits: enough workgroups for two per CU, but at least one key tile per wave in each.
 struct AttnLaunch { bool wide, shared; int DP, RT, row_blocks, key_waves, splits; int64_t ws; };
 AttnLaunch attn_launch(const vox_hip_tree_attn_t *a) {
@@ -165,12 +165,12 @@ AttnLaunch attn_launch(const vox_hip_tree_attn_t *a) {
     if (!l.wide || a->batch == 0 || a->nodes == 0) return l;
     const int64_t R = (int64_t)a->nodes * (a->heads / a->kv_heads);
     l.DP = a->head_dim <= 64 ? 64 : a->head_dim <= 128 ? 128 : 256;
-    l.shared = R > (l.DP == 256 ? 16 : 32);
+    l.shared = R > (l.DP > 64 ? 16 : 32);
     l.RT = l.DP == 256 || R <= 16 || (l.shared && R <= 64) ? 1 : 2;
     const int rows = l.RT * 16 * (l.shared ? ATTN_WAVES : 1);
     l.key_waves = l.shared ? 1 : ATTN_WAVES;
     l.row_blocks = (int)((R + rows - 1) / rows);
-    const int KT = a->dtype == VOX_F32 ? 16 : 32;
+    const int KT = a->dtype == VOX_F32 && !l.shared ? 16 : 32;
     const int64_t keys = a->window > 0 ? std::min(a->cap, a->window) : a->cap, tiles = (keys + KT - 1) / KT + (a->nodes + KT - 1) / KT;
     const int64_t groups = (int64_t)a->batch * a->kv_heads * l.row_blocks;
     l.splits = (int)std::max<int64_t>(1, std::min<int64_t>({64, 512 / groups, (tiles + l.key_waves - 1) / l.key_waves}));
@@ -180,6 +180,12 @@ AttnLaunch attn_launch(const vox_hip_tree_attn_t *a) {
 template <typename T, int DP, int RT, bool SHARED> void launch_attn2(const TreeAttnArgs &t, const TreeAttnPlan &p, dim3 grid, hipStream_t s) {
     hipLaunchKernelGGL((k_tree_attn<T, DP, RT, SHARED>), grid, dim3(64 * ATTN_WAVES), (attn_lds<T, DP, RT, SHARED>()), s, t, p);
 }
+template <typename T, bool SHARED> void launch_attn_join(const TreeAttnArgs &t, const TreeAttnPlan &p, int DP, int batch, hipStream_t s) {
+    const dim3 grid((t.T * t.G + 3) / 4, t.Hk, batch);
+    if (DP == 64) hipLaunchKernelGGL((k_tree_attn_join<T, 16, SHARED>), grid, dim3(256), 0, s, t, p);
+    else if (DP == 128) hipLaunchKernelGGL((k_tree_attn_join<T, 32, SHARED>), grid, dim3(256), 0, s, t, p);
+    else hipLaunchKernelGGL((k_tree_attn_join<T, 64, SHARED>), grid, dim3(256), 0, s, t, p);
+}
 template <typename T, int DP> void launch_attn(const TreeAttnArgs &t, const TreeAttnPlan &p, const AttnLaunch &l, dim3 grid, hipStream_t s) {
     if constexpr (DP == 256) {
         if (l.shared) launch_attn2<T, DP, 1, true>(t, p, grid, s);
@@ -187,8 +193,8 @@ template <typename T, int DP> void launch_attn(const TreeAttnArgs &t, const Tree
     } else {
         if (l.shared && l.RT == 2) launch_attn2<T, DP, 2, true>(t, p, grid, s);
         else if (l.shared) launch_attn2<T, DP, 1, true>(t, p, grid, s);
-        else if (l.RT == 2) launch_attn2<T, DP, 2, false>(t, p, grid, s);
-        else launch_attn2<T, DP, 1, false>(t, p, grid, s);
+        else if (l.RT == 1) launch_attn2<T, DP, 1, false>(t, p, grid, s);
+        else if constexpr (DP == 64) launch_attn2<T, DP, 2, false>(t, p, grid, s);
     }
 }
 }  // namespace
@@ -224,10 +230,8 @@ extern "C" int vox_hip_tree_attention(const vox_hip_tree_attn_t *a, void *ws, si
         if (l.DP == 64) launch_attn<T, 64>(t, p, l, grid, s);
         else if (l.DP == 128) launch_attn<T, 128>(t, p, l, grid, s);
         else launch_attn<T, 256>(t, p, l, grid, s);
-        const dim3 rows((R + 3) / 4, a->kv_heads, a->batch);
-        if (l.splits > 1 && l.DP == 64) hipLaunchKernelGGL((k_tree_attn_join<T, 16>), rows, dim3(256), 0, s, t, p, l.key_waves);
-        else if (l.splits > 1 && l.DP == 128) hipLaunchKernelGGL((k_tree_attn_join<T, 32>), rows, dim3(256), 0, s, t, p, l.key_waves);
-        else if (l.splits > 1) hipLaunchKernelGGL((k_tree_attn_join<T, 64>), rows, dim3(256), 0, s, t, p, l.key_waves);
+        if (l.splits > 1 && l.shared) launch_attn_join<T, true>(t, p, l.DP, a->batch, s);
+        else if (l.splits > 1) launch_attn_join<T, false>(t, p, l.DP, a->batch, s);
     });
     return launched("vox_hip_tree_attention");
 }

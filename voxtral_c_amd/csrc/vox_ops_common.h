@@ -23,8 +23,10 @@ template <typename T, int N> __device__ __forceinline__ void load_vec(float (&o)
 // glds16 (vox_common.h) from a wave-uniform address and a 32-bit offset per lane.
 __device__ __forceinline__ void glds16_at(const void *base, unsigned offset, unsigned lds_base) {
     unsigned keep;
+    const uint64_t b = (uint64_t)base;
+    const uint64_t u = ((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)b);
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "v"(offset), "s"(base), "s"(lds_base) : "memory");
+                 : "=&s"(keep) : "v"(offset), "s"(u), "s"(lds_base) : "memory");
 }
 
 __device__ __forceinline__ int wave_sum_i(int v) {

@@ -1,5 +1,6 @@
 // vox_tree_attn.h — attention of the nodes of a draft tree over a ring cache and over their own ancestors.
 #pragma once
+#include <type_traits>
 #include "vox_ops_common.h"
 
 namespace vox {
@@ -103,7 +104,7 @@ template <typename T> __global__ __launch_bounds__(256) void k_tree_attn_scalar(
 // long cache by k_tree_attn_join.
 template <typename T> struct AttnType;
 template <> struct AttnType<float> {
-    static constexpr int KT = 16, SHIFT = 0;
+    static constexpr int SHIFT = 0;
     typedef unsigned Bits;
     static constexpr Bits INF = 0x7f800000u, SIGN = 0x80000000u;
     static constexpr float LAZY = 8.f;
@@ -111,7 +112,7 @@ template <> struct AttnType<float> {
 // P is rounded to bf16 in front of its product (a half step of 2^-8 per weight, like the rounding of the output itself): the product then runs at
 // the 16-bit rate.  The weights' sum is taken of the f32 values.
 template <> struct AttnType<bf16_t> {
-    static constexpr int KT = 32, SHIFT = 0;
+    static constexpr int SHIFT = 0;
     typedef unsigned short Bits;
     static constexpr Bits INF = 0x7f80, SIGN = 0x8000;
     static constexpr float LAZY = 8.f;
@@ -119,13 +120,19 @@ template <> struct AttnType<bf16_t> {
 // f16: the same with a half step of 2^-11; weights are lifted by 2^12 so that what is 2^-26 of the largest one is still a normal number (a sum over
 // tens of thousands of small weights would lose them otherwise).
 template <> struct AttnType<f16_t> {
-    static constexpr int KT = 32, SHIFT = 12;
+    static constexpr int SHIFT = 12;
     typedef unsigned short Bits;
     static constexpr Bits INF = 0x7c00, SIGN = 0x8000;
     static constexpr float LAZY = 3.f;
 };
 
-constexpr int ATTN_WAVES = 4, ATTN_STAGES = 3;
+constexpr int ATTN_WAVES = 4;
+// Shared keys of f32 are multiplied on the bf16 pipe: a number is exactly the sum of three bf16 ones (8 of its 24 bits each), and of the nine
+// products the six down to 2^-16 of the largest are taken, the rest is below 2^-24.  An f32 matrix instruction takes the vector unit's cycles (measured:
+// the two run one after the other, 0.23 + 0.23 ms -> 0.46 ms), a bf16 one does not, and six of them take 6 x 17 cycles where f32 takes 8 x 33.
+template <typename T, bool SHARED> constexpr bool ATTN_SPLIT = SHARED && sizeof(T) == 4;
+template <typename T, bool SHARED> constexpr int ATTN_KT = SHARED || sizeof(T) == 2 ? 32 : 16;              // keys of a step
+template <typename T> constexpr int ATTN_STAGES = sizeof(T) == 4 ? 2 : 3;                                   // (two workgroups per CU)
 struct TreeAttnPlan {
     int splits, row_blocks;
     float *part_o, *part_ml;      // [splits][batch * Hk][rows][D], [splits][batch * Hk][rows][2]
@@ -154,6 +161,33 @@ template <typename T, typename V> __device__ __forceinline__ f32x4 attn_mma(cons
     else return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, acc, 0, 0, 0);
 }
 
+// Eight numbers of f32 as three bf16 operands: x = h + m + l exactly (each step takes the number's top 8 bits and leaves the rest).
+template <typename V, typename F> __device__ __forceinline__ void split3(F x, V &h, V &m, V &l) {
+    typedef unsigned words __attribute__((ext_vector_type(4)));
+    words hw, mw, lw;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float a = x(2 * i), b = x(2 * i + 1);
+        hw[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);          // the upper halves of b and a
+        const float a1 = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u), b1 = b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+        mw[i] = __builtin_amdgcn_perm(__float_as_uint(b1), __float_as_uint(a1), 0x07060302u);
+        const float a2 = a1 - __uint_as_float(__float_as_uint(a1) & 0xffff0000u), b2 = b1 - __uint_as_float(__float_as_uint(b1) & 0xffff0000u);
+        lw[i] = __builtin_amdgcn_perm(__float_as_uint(b2), __float_as_uint(a2), 0x07060302u);
+    }
+    h = __builtin_bit_cast(V, hw);
+    m = __builtin_bit_cast(V, mw);
+    l = __builtin_bit_cast(V, lw);
+}
+// acc + x y of split numbers, smallest products first.
+template <typename V> __device__ __forceinline__ f32x4 split_mma(const V (&x)[3], const V (&y)[3], f32x4 acc) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[2], y[0], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], y[2], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[1], y[1], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[1], y[0], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], y[1], acc, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], y[0], acc, 0, 0, 0);
+}
+
 // Key tiles of a sequence: the cache's, then the tree's; split s takes tiles [s * per, (s + 1) * per).
 struct TileRange {
     int64_t first, len;
@@ -178,17 +212,21 @@ struct KeyTile {
 
 // Bytes of LDS of a workgroup: the stages (shared) or Q^T (own, where registers do not hold it), later the outputs; and maxima and sums.
 template <typename T, int DP, int RT, bool SHARED> constexpr int attn_lds() {
-    const int rows = RT * 16 * (SHARED ? ATTN_WAVES : 1), out = rows * (DP + 4) * 4, stages = SHARED ? ATTN_STAGES * 2 * AttnType<T>::KT * DP * (int)sizeof(T) : 0;
+    const int rows = RT * 16 * (SHARED ? ATTN_WAVES : 1), out = rows * (DP + 4) * 4, stages = SHARED ? ATTN_STAGES<T> * 2 * ATTN_KT<T, SHARED> * DP * (int)sizeof(T) : 0;
     return (out > stages ? out : stages) + 2 * (SHARED ? 1 : ATTN_WAVES) * rows * 4;
 }
 
 template <typename T, int DP, int RT, bool SHARED>
-__global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_attn(TreeAttnArgs a, TreeAttnPlan plan) {
+__global__ __launch_bounds__(64 * ATTN_WAVES, (DP == 256 || (ATTN_SPLIT<T, SHARED> && DP * RT > 128) ? 1 : 2)) void k_tree_attn(TreeAttnArgs a, TreeAttnPlan plan) {
     typedef AttnType<T> A;
     typedef typename A::Bits bits_t;
-    constexpr int KT = A::KT, E = DP / 16, NK = KT / 16, VK = KT / 4;            // VK: keys per lane of a V operand
+    constexpr bool SPLIT = ATTN_SPLIT<T, SHARED>;
+    constexpr int KT = ATTN_KT<T, SHARED>, STAGES = ATTN_STAGES<T>, E = DP / 16, NK = KT / 16, VK = KT / 4;      // VK: keys per lane of a V operand
     constexpr int U = sizeof(T) == 2 ? 8 : 4;                                    // elements per 16-byte load
     constexpr int KS = DP / (4 * U);                                             // K / Q loads per lane and 16 keys / rows
+    typedef typename std::conditional<SPLIT, bf16_t, T>::type M;                 // what the matrix instructions take, MU values per lane
+    constexpr int MU = sizeof(M) == 2 ? 8 : 4, MS = DP / (4 * MU);               // MS: steps over the dimensions
+    typedef M mvec __attribute__((ext_vector_type(MU)));
     constexpr int VU = E < U ? E : U, VL = E / VU;                               // V: VL loads of VU elements per key
     constexpr float LOG2E = 1.44269504088896340736f;
     typedef T kvec __attribute__((ext_vector_type(U)));
@@ -215,7 +253,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
 
     // this lane's query rows; a negative scale goes into Q's sign
     constexpr bool QLDS = !SHARED && (sizeof(T) == 4 || DP == 256);
-    kvec qf[QLDS ? 1 : RT][QLDS ? 1 : KS];
+    mvec qf[QLDS ? 1 : RT][QLDS ? 1 : MS][SPLIT ? 3 : 1];
     kvec *qs = reinterpret_cast<kvec *>(lds);                // [RT][KS][64 lanes]
     int row_depth[RT], row_node[RT];
 #pragma unroll
@@ -224,14 +262,19 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
         row_node[t] = node;
         row_depth[t] = row < R ? a.depth[(size_t)b * a.T + node] : -1;
         const T *q = (const T *)a.q + b * a.q_sb + node * a.q_st + h * a.q_sh;
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-            const int d = s * 4 * U + c * U;
+        auto load = [&](int d) {
             kvec x = kvec(T(0.f));
             if (row < R && d < a.D) x = *reinterpret_cast<const kvec *>(q + d);
-            if (a.scale < 0.f) x = -x;
-            if constexpr (!QLDS) qf[t][s] = x;
-            else if (kw == 0) qs[(t * KS + s) * 64 + lane] = x;
+            return a.scale < 0.f ? -x : x;
+        };
+#pragma unroll
+        for (int s = 0; s < MS; s++) {
+            const int d = s * 4 * MU + c * MU;
+            if constexpr (SPLIT) {
+                const kvec x[2] = {load(d), load(d + 4)};
+                split3<mvec>([&](int i) { return x[i >> 2][i & 3]; }, qf[t][s][0], qf[t][s][1], qf[t][s][2]);
+            } else if constexpr (!QLDS) qf[t][s][0] = load(d);
+            else if (kw == 0) qs[(t * KS + s) * 64 + lane] = load(d);
         }
     }
     const float scale2 = fabsf(a.scale) * LOG2E;
@@ -367,6 +410,18 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
         }
     };
 
+    auto read_v = [&](const char *sv, int from, int to) {
+#pragma unroll
+        for (int j = 0; j < VK; j++) {
+            const int key = (j >> 2) * 16 + c * 4 + (j & 3);
+#pragma unroll
+            for (int u = 0; u < VL; u++) {
+                const int at = (u * 16 + n16) * VU * (int)sizeof(T);             // byte of the row
+                if (u >= from && u < to) vf[j][u] = *reinterpret_cast<const vvec *>(sv + piece_at(key, at >> 4) + (at & 15));
+            }
+        }
+    };
+
     f32x4 o[RT][E];
     float m[RT], l[RT];
 #pragma unroll
@@ -376,21 +431,15 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
         for (int e = 0; e < E; e++) o[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     bool bad = false;                                        // a masked tile held a value that is not finite
-    auto v_operand = [&](int e) {
-        kvec av;
-#pragma unroll
-        for (int j = 0; j < VK; j++) av[j] = vf[j][e / VU][e % VU];
-        return av;
-    };
 
     int t = SHARED ? t_begin : t_begin + kw, stage = 0;
     if constexpr (SHARED) {
         if (a.D < DP) {                                      // dimensions that no load fills
-            for (int i = tid; i < ATTN_STAGES * 2 * TILE / 16; i += 64 * ATTN_WAVES) reinterpret_cast<uint4 *>(lds)[i] = uint4{0, 0, 0, 0};
+            for (int i = tid; i < STAGES * 2 * TILE / 16; i += 64 * ATTN_WAVES) reinterpret_cast<uint4 *>(lds)[i] = uint4{0, 0, 0, 0};
             __syncthreads();
         }
 #pragma unroll
-        for (int i = 0; i < ATTN_STAGES - 1; i++)
+        for (int i = 0; i < STAGES - 1; i++)
             if (t + i < t_end) issue(t + i, i);
     } else {
         if (QLDS) __syncthreads();
@@ -403,12 +452,12 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
             // Tile t has landed when at most the next tile's loads are in flight; behind the barrier everyone's has, and everyone is done with the
             // tile that the next loads overwrite (their LDS reads have returned: the compiler may place the products behind the barrier).  Only of a
             // whole tile it is certain that every wave has issued all its loads.
-            if (more && a.D == DP && t + 1 < full_end) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
+            if (STAGES == 3 && more && a.D == DP && t + 1 < full_end) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (t + ATTN_STAGES - 1 < t_end) issue(t + ATTN_STAGES - 1, stage == 0 ? ATTN_STAGES - 1 : stage - 1);
+            if (t + STAGES - 1 < t_end) issue(t + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
             sk = lds + stage * (2 * TILE);
             sv = sk + TILE;
-            stage = stage == ATTN_STAGES - 1 ? 0 : stage + 1;
+            stage = stage == STAGES - 1 ? 0 : stage + 1;
         }
         if constexpr (SHARED) {
             // 0 * inf: a value that is not finite must not reach the rows that do not see its key, nor what lies behind the last key.  Such values become
@@ -430,29 +479,35 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
             }
             if (idle) continue;
         }
-        kvec pf[RT];                                         // the row tiles' weights as the second product's operand
+        mvec pf[RT][SPLIT ? 3 : 1];                          // the row tiles' weights as the second product's operand
         f32x4 s[RT][NK];
         if constexpr (SHARED) {
             // (all of K first, V as soon as the scores are under way: no product waits for LDS)
-            kvec kk[NK][KS];
-#pragma unroll
-            for (int i = 0; i < NK; i++)
-#pragma unroll
-                for (int x = 0; x < KS; x++) kk[i][x] = *reinterpret_cast<const kvec *>(sk + piece_at(i * 16 + n16, x * 4 + c));
-#pragma unroll
-            for (int x = 0; x < KS; x++)
+            if constexpr (SPLIT) {
 #pragma unroll
                 for (int i = 0; i < NK; i++)
 #pragma unroll
-                    for (int r = 0; r < RT; r++) s[r][i] = attn_mma<T>(kk[i][x], qf[r][x], x == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[r][i]);
+                    for (int x = 0; x < MS; x++) {
+                        const kvec k[2] = {*reinterpret_cast<const kvec *>(sk + piece_at(i * 16 + n16, x * 8 + c * 2)),
+                                           *reinterpret_cast<const kvec *>(sk + piece_at(i * 16 + n16, x * 8 + c * 2 + 1))};
+                        mvec kp[3];
+                        split3<mvec>([&](int j) { return k[j >> 2][j & 3]; }, kp[0], kp[1], kp[2]);
 #pragma unroll
-            for (int j = 0; j < VK; j++) {
-                const int key = (j >> 2) * 16 + c * 4 + (j & 3);
+                        for (int r = 0; r < RT; r++) s[r][i] = split_mma(kp, qf[r][x], x == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[r][i]);
+                    }
+            } else {
+                kvec kk[NK][KS];
 #pragma unroll
-                for (int u = 0; u < VL; u++) {
-                    const int at = (u * 16 + n16) * VU * (int)sizeof(T);         // byte of the row
-                    vf[j][u] = *reinterpret_cast<const vvec *>(sv + piece_at(key, at >> 4) + (at & 15));
-                }
+                for (int i = 0; i < NK; i++)
+#pragma unroll
+                    for (int x = 0; x < KS; x++) kk[i][x] = *reinterpret_cast<const kvec *>(sk + piece_at(i * 16 + n16, x * 4 + c));
+#pragma unroll
+                for (int x = 0; x < KS; x++)
+#pragma unroll
+                    for (int i = 0; i < NK; i++)
+#pragma unroll
+                        for (int r = 0; r < RT; r++) s[r][i] = attn_mma<T>(kk[i][x], qf[r][x][0], x == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[r][i]);
+                read_v(sv, 0, VL);
             }
         }
 #pragma unroll
@@ -465,7 +520,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
                     for (int x = 0; x < KS; x++) {
                         kvec q;
                         if constexpr (QLDS) q = qs[(r * KS + x) * 64 + lane];
-                        else q = qf[r][x];
+                        else q = qf[r][x][0];
                         s[r][i] = attn_mma<T>(kf[i][x], q, s[r][i]);
                     }
                 }
@@ -497,10 +552,13 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
             for (int i = 0; i < NK; i++)
 #pragma unroll
                 for (int y = 0; y < 4; y++) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(s[r][i][y], scale2, -base));
-                    l[r] += p;
-                    pf[r][i * 4 + y] = from_f32<T>(p);
+                    s[r][i][y] = __builtin_amdgcn_exp2f(fmaf(s[r][i][y], scale2, -base));
+                    l[r] += s[r][i][y];
                 }
+            if constexpr (SPLIT) split3<mvec>([&](int i) { return s[r][i >> 2][i & 3]; }, pf[r][0], pf[r][1], pf[r][2]);
+            else
+#pragma unroll
+                for (int i = 0; i < MU; i++) pf[r][0][i] = from_f32<M>(s[r][i >> 2][i & 3]);
         }
         if constexpr (!SHARED) {
             if (more) load_k(t + KW);
@@ -515,9 +573,19 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
         // O^T += V^T P^T
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            const kvec av = v_operand(e);
+            if constexpr (SPLIT) {
+                if (e % VU == 0) read_v(sv, e / VU, e / VU + 1);
+                mvec av[3];
+                split3<mvec>([&](int j) { return vf[j][e / VU][e % VU]; }, av[0], av[1], av[2]);
 #pragma unroll
-            for (int r = 0; r < RT; r++) o[r][e] = attn_mma<T>(av, pf[r], o[r][e]);
+                for (int r = 0; r < RT; r++) o[r][e] = split_mma(av, pf[r], o[r][e]);
+            } else {
+                mvec av;
+#pragma unroll
+                for (int j = 0; j < VK; j++) av[j] = vf[j][e / VU][e % VU];
+#pragma unroll
+                for (int r = 0; r < RT; r++) o[r][e] = attn_mma<M>(av, pf[r][0], o[r][e]);
+            }
         }
         if constexpr (!SHARED) {
             if (more) load_v(t + KW);
@@ -536,18 +604,18 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
 #pragma unroll
                 for (int r = 0; r < RT; r++) {
                     const unsigned sees = visible(t, tile_at(t).count, r);
-                    kvec one;
+                    mvec one;
 #pragma unroll
-                    for (int j = 0; j < VK; j++) one[j] = (sees >> ((j >> 2) * 16 + c * 4 + (j & 3))) & 1u ? T(1.f) : T(0.f);
+                    for (int j = 0; j < VK; j++) one[j] = (sees >> ((j >> 2) * 16 + c * 4 + (j & 3))) & 1u ? M(1.f) : M(0.f);
 #pragma unroll
                     for (int e = 0; e < E; e++) {
-                        kvec is;
+                        mvec is;
 #pragma unroll
                         for (int j = 0; j < VK; j++) {
                             const bits_t x = bits_of(vf[j][e / VU][e % VU]);
-                            is[j] = (kind == 2 ? (bits_t)(x & ~A::SIGN) > A::INF : x == inf) ? T(1.f) : T(0.f);
+                            is[j] = (kind == 2 ? (bits_t)(x & ~A::SIGN) > A::INF : x == inf) ? M(1.f) : M(0.f);
                         }
-                        const f32x4 n = attn_mma<T>(is, one, f32x4{0.f, 0.f, 0.f, 0.f});
+                        const f32x4 n = attn_mma<M>(is, one, f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
                         for (int y = 0; y < 4; y++)
                             if (n[y] > 0.f) o[r][e][y] += value;
@@ -616,11 +684,11 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, DP == 256 ? 1 : 2) void k_tree_att
 
 // Joins the parts of a row: one wave per (row, kv head, sequence); grid (ceil(rows / 4), Hk, batch).  L lanes take one part's outputs, four values
 // each (the matrix-pipe form's head_dim is a multiple of four), 64 / L parts at a time, their weights first: bound by the read of the parts.
-template <typename T, int L> __global__ __launch_bounds__(256) void k_tree_attn_join(TreeAttnArgs a, TreeAttnPlan plan, int key_waves) {
+template <typename T, int L, bool SHARED> __global__ __launch_bounds__(256) void k_tree_attn_join(TreeAttnArgs a, TreeAttnPlan plan) {
     typedef AttnType<T> A;
     const int lane = threadIdx.x & 63, R = a.T * a.G, row = blockIdx.x * 4 + (threadIdx.x >> 6), kvh = blockIdx.y, b = blockIdx.z;
     if (row >= R) return;
-    const TileRange tr = tile_range<A::KT>(a, b, plan.splits, key_waves);
+    const TileRange tr = tile_range<ATTN_KT<T, SHARED>>(a, b, plan.splits, SHARED ? 1 : ATTN_WAVES);
     const int n = (tr.n_all + tr.per - 1) / tr.per;          // at most 64 parts: lane s holds part s's weight
     if (n <= 1) return;                                      // written by its only part
     const int64_t step = (int64_t)gridDim.z * a.Hk * R, at = ((int64_t)b * a.Hk + kvh) * R + row;
