@@ -146,9 +146,10 @@ template <typename T, int MT> __global__ __launch_bounds__(64 * I8_ROWS_WAVES) v
 // ---- many rows: a matrix product ------------------------------------------------------------------------------------------------
 // BM rows x 128 channels per workgroup of four waves (2 x 2, each BM / 2 rows x 64 channels) on v_mfma_i32_32x32x32_i8.  Slices of 128 bytes of K
 // go from memory into LDS without registers (global_load_lds_dwordx4: a wave's instruction brings 128 bytes of each of 8 rows), STAGES of them in
-// flight with one barrier per slice.  16-byte pieces of a row are stored at (piece ^ (row & 7)): the MFMA operand reads (lane = row, one piece) then
-// touch every bank once.  Outputs leave through LDS so that rows are written in whole lines.
+// flight with one barrier per slice.  16-byte pieces of a row are stored at (piece ^ (row / 2 % 8)): of the MFMA operand reads (lane = row, one
+// piece) 16 lanes at a time then touch every one of the 64 banks once (with row % 8 the counters show a conflict on every second cycle).  Outputs leave through LDS so that rows are written in whole lines.
 constexpr int I8_BN = 128, I8_BK = 128;
+__device__ __forceinline__ int i8_swizzle(int row) { return (row >> 1) & 7; }
 template <typename T, int BM, int STAGES> constexpr unsigned i8_tile_lds() {        // stages, later outputs; scales and bias behind them
     const unsigned stages = STAGES * (BM + I8_BN) * I8_BK, out = BM * (I8_BN * (unsigned)sizeof(T) + 16);
     return (stages > out ? stages : out) + (BM + 2 * I8_BN) * 4;
@@ -172,7 +173,7 @@ template <typename T, int BM, int STAGES> __global__ __launch_bounds__(256) void
     const int8_t *src[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; i++) {
-        const int row = (i * 4 + wave) * 8 + (lane >> 3), p = piece ^ (row & 7);
+        const int row = (i * 4 + wave) * 8 + (lane >> 3), p = piece ^ i8_swizzle(row);
         src[i] = i * 32 >= BM ? a.w + (int64_t)min(n0 + row - BM, a.N - 1) * a.w_stride + p * 16 : a.xq + (int64_t)min(m0 + row, a.M - 1) * a.ldq + p * 16;
     }
     const int slices = a.ldq / I8_BK;
@@ -182,7 +183,7 @@ template <typename T, int BM, int STAGES> __global__ __launch_bounds__(256) void
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
             if (i < from || i >= to) continue;
-            const int row = (i * 4 + wave) * 8 + (lane >> 3), p = (piece ^ (row & 7)) * 16;
+            const int row = (i * 4 + wave) * 8 + (lane >> 3), p = (piece ^ i8_swizzle(row)) * 16;
             const bool past = i * 32 >= BM && s * I8_BK + p >= a.K;
             glds16(src[i] + (past ? -p : s * I8_BK), __builtin_amdgcn_readfirstlane(base + (i * 4 + wave) * 1024));
         }
@@ -214,12 +215,12 @@ template <typename T, int BM, int STAGES> __global__ __launch_bounds__(256) void
 #pragma unroll
             for (int j = 0; j < NJ; j++) {
                 const int row = BM + wn * 64 + j * 32 + (lane & 31);
-                wf[k & 1][j] = *reinterpret_cast<const i32x4 *>(buf + row * I8_BK + ((q ^ (row & 7)) << 4));
+                wf[k & 1][j] = *reinterpret_cast<const i32x4 *>(buf + row * I8_BK + ((q ^ i8_swizzle(row)) << 4));
             }
 #pragma unroll
             for (int i = 0; i < MI; i++) {
                 const int row = wm * (BM / 2) + i * 32 + (lane & 31);
-                xf[k & 1][i] = *reinterpret_cast<const i32x4 *>(buf + row * I8_BK + ((q ^ (row & 7)) << 4));
+                xf[k & 1][i] = *reinterpret_cast<const i32x4 *>(buf + row * I8_BK + ((q ^ i8_swizzle(row)) << 4));
             }
         };
         read(0);

@@ -382,18 +382,19 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, (DP == 256 || (ATTN_SPLIT<T, SHARE
         }
     };
 
-    // ---- keys in LDS: per stage K [KT][DP], V [KT][DP]; 16-byte piece q of row r sits at (q ^ (r & 7)), so that the 8 lanes of one access (8 rows, one
-    // piece each) touch every bank once
+    // ---- keys in LDS: per stage K [KT][DP], V [KT][DP]; 16-byte piece q of row r sits at q ^ swizzle(r): 16 lanes of an access (16 rows, one piece each)
+    // touch every one of the 64 banks once
     constexpr int PIECES = DP * (int)sizeof(T) / 16, TILE = KT * DP * (int)sizeof(T), LOADS = TILE / (1024 * ATTN_WAVES);        // LOADS: per wave, for K and for V
     static_assert(TILE % (1024 * ATTN_WAVES) == 0, "a tile is a whole number of a workgroup's loads");
-    auto piece_at = [](int row, int q) { return (row * PIECES + (q ^ (row & 7))) * 16; };
+    auto swizzle = [](int row) { return PIECES >= 16 ? row & 15 : (row >> 1) & 7; };
+    auto piece_at = [&](int row, int q) { return (row * PIECES + (q ^ swizzle(row))) * 16; };
     auto issue = [&](int t, int stage) {
         const unsigned base = lds_addr(lds) + (unsigned)stage * (2 * TILE);
         if (is_plain(t)) {
             const char *k = kc + (int64_t)slot_of(t) * ks, *v = vc + (int64_t)slot_of(t) * vs;
 #pragma unroll
             for (int i = 0; i < LOADS; i++) {
-                const int at = (i * ATTN_WAVES + wave) * 64, row = (at + lane) / PIECES, q = ((at + lane) % PIECES) ^ (row & 7);
+                const int at = (i * ATTN_WAVES + wave) * 64, row = (at + lane) / PIECES, q = ((at + lane) % PIECES) ^ swizzle(row);
                 glds16_at(k, (unsigned)(row * ks + q * 16), __builtin_amdgcn_readfirstlane(base + at * 16));
                 glds16_at(v, (unsigned)(row * vs + q * 16), __builtin_amdgcn_readfirstlane(base + TILE + at * 16));
             }
@@ -402,7 +403,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, (DP == 256 || (ATTN_SPLIT<T, SHARE
         const KeyTile x = tile_at(t);
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
-            const int at = (i * ATTN_WAVES + wave) * 64, row = (at + lane) / PIECES, q = ((at + lane) % PIECES) ^ (row & 7), from = row < x.wrap ? row : row - x.cap;
+            const int at = (i * ATTN_WAVES + wave) * 64, row = (at + lane) / PIECES, q = ((at + lane) % PIECES) ^ swizzle(row), from = row < x.wrap ? row : row - x.cap;
             if (row < x.count && q * U < a.D) {
                 glds16(x.k + (int64_t)from * x.ks + q * 16, __builtin_amdgcn_readfirstlane(base + at * 16));
                 glds16(x.v + (int64_t)from * x.vs + q * 16, __builtin_amdgcn_readfirstlane(base + TILE + at * 16));
