@@ -389,7 +389,7 @@ def test_token_scores_nothing():
 
 # ---- 8-bit integers ----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
-@pytest.mark.parametrize("R,K", [(1, 1), (3, 64), (2, 1000), (5, 4099), (300, 128)])
+@pytest.mark.parametrize("R,K", [(1, 1), (3, 64), (2, 1000), (5, 4099), (300, 128), (2, 4096), (3, 4100), (2, 8192), (2, 8200), (1, 20000)])
 def test_quantize_rows(dtype, R, K):
     rng = np.random.default_rng(R * K)
     x = randn(rng, R, K, dtype=dtype, scale=10.0)
@@ -432,7 +432,7 @@ def check_linear(x, w, ws, bias, dtype):
 
 I8 = [(1, 64, 16), (1, 1280, 6144), (2, 100, 7), (3, 1, 5), (5, 128, 1000), (16, 256, 48), (17, 320, 130), (25, 5120, 1280), (33, 80, 64), (64, 4096, 33), (65, 1008, 257), (130, 192, 96),
       (200, 1280, 520), (257, 2064, 129), (1000, 64, 65), (300, 77, 200), (128, 128, 128), (256, 512, 256), (513, 640, 768),
-      (700, 144, 5500), (1030, 208, 8000)]
+      (700, 144, 5500), (1030, 208, 8000), (33, 2048, 300), (64, 5120, 1280), (70, 1536, 2000), (129, 4096, 1000), (40, 640, 127), (16, 1024, 100), (4, 4096, 65), (13, 1248, 96), (1, 16384, 40)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])

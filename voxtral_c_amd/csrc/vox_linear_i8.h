@@ -28,7 +28,7 @@ __device__ __forceinline__ RowScale row_scale(unsigned amax_bits) {
 }
 
 // One workgroup per row: q [rows, ldq] (columns K .. ldq - 1 are zeros), scale [rows].  Bound by the row's two trips (the second one hits the
-// caches).  N elements per load: K, stride and x allow it, and ldq % N = 0.
+// caches; keeping the row in registers instead measured the same).  N elements per load: K, stride and x allow it, and ldq % N = 0.
 template <typename T, int N> __global__ __launch_bounds__(256) void k_quant_rows_i8(const T *x, int64_t stride, int K, int ldq, int8_t *q, float *scale) {
     __shared__ unsigned red[4];
     const int64_t row = blockIdx.x;
@@ -67,6 +67,8 @@ struct LinearI8Args {
     void *y;
     int64_t y_stride;
     int M, K, N, ldq;
+    int *part;                   // [splits, padded rows, padded channels]: sums of a part of K each, where K is split
+    int splits;
 };
 // Three roundings of f32 (the sum's conversion and two products) and the one to the output's type; the sum itself is exact.
 __device__ __forceinline__ float i8_scaled(int acc, float xs, float ws) { return ((float)acc * ws) * xs; }
@@ -143,6 +145,68 @@ template <typename T, int MT> __global__ __launch_bounds__(64 * I8_ROWS_WAVES) v
     }
 }
 
+// The same in one launch for a few rows (single tokens): every workgroup quantises all of x into its LDS while its first weights are on their way.  Up
+// to I8_FEW elements of x: 32 per thread, about a microsecond; a launch of its own costs 3 us (1 x 1280 x 6144, f32: 13.9 -> 10.9 us a call).
+constexpr int I8_FEW = 16384, I8_FEW_ROWS = 16, I8_FEW_AHEAD = 2;
+template <typename T, int N> __global__ __launch_bounds__(64 * I8_ROWS_WAVES) void k_linear_i8_few(LinearI8Args a, const T *x, int64_t x_stride) {
+    __shared__ i32x4 part[I8_ROWS_WAVES][64];
+    __shared__ float xs[I8_FEW_ROWS];
+    extern __shared__ __attribute__((aligned(128))) char lds[];                  // xq [M][ldq + 16]: rows start on different banks
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, c = lane >> 4;
+    const int n0 = blockIdx.x * 16, ld = a.ldq + 16;
+    const int8_t *w = a.w + (int64_t)min(n0 + n16, a.N - 1) * a.w_stride + c * 16;
+    auto weights = [&](int k) { return *reinterpret_cast<const i32x4 *>(w + (k + c * 16 < a.K ? k : -c * 16)); };       // (see above)
+    i32x4 ahead[I8_FEW_AHEAD][2];
+#pragma unroll
+    for (int i = 0; i < I8_FEW_AHEAD; i++) {
+        const int k = (wave + i * I8_ROWS_WAVES) * 128;
+        if (k < a.K) { ahead[i][0] = weights(k); ahead[i][1] = weights(k + 64); }
+    }
+    for (int row = wave; row < a.M; row += I8_ROWS_WAVES) {
+        const T *xr = x + row * x_stride;
+        unsigned m = 0;
+        for (int k = lane * N; k < a.K; k += 64 * N) {
+            float v[N];
+            load_vec<T, N>(v, xr + k);
+#pragma unroll
+            for (int i = 0; i < N; i++) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+        }
+        const RowScale r = row_scale(wave_max_u(m));
+        for (int k = lane * N; k < a.ldq; k += 64 * N) {
+            typedef int8_t out __attribute__((ext_vector_type(N)));
+            float v[N] = {};
+            out o;
+            if (k < a.K && !r.broken) load_vec<T, N>(v, xr + k);
+#pragma unroll
+            for (int i = 0; i < N; i++) o[i] = (int8_t)(int)quant_i8(v[i], r.s, r.inv);
+            *reinterpret_cast<out *>(lds + row * ld + k) = o;
+        }
+        if (lane == 0) xs[row] = r.broken ? NAN : r.s;
+    }
+    __syncthreads();
+    const char *xq = lds + min(n16, a.M - 1) * ld + c * 16;
+    i32x4 acc = {};
+    auto step = [&](int k, i32x4 w0, i32x4 w1) {
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w0, *reinterpret_cast<const i32x4 *>(xq + k), acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w1, *reinterpret_cast<const i32x4 *>(xq + k + 64), acc, 0, 0, 0);
+    };
+#pragma unroll
+    for (int i = 0; i < I8_FEW_AHEAD; i++) {
+        const int k = (wave + i * I8_ROWS_WAVES) * 128;
+        if (k < a.K) step(k, ahead[i][0], ahead[i][1]);
+    }
+    for (int k = (wave + I8_FEW_AHEAD * I8_ROWS_WAVES) * 128; k < a.K; k += 128 * I8_ROWS_WAVES) step(k, weights(k), weights(k + 64));
+    part[wave][lane] = acc;
+    __syncthreads();
+    if (tid < 256) {
+        const int ch = tid & 15, row = tid >> 4, n = n0 + ch;
+        int sum = 0;
+#pragma unroll
+        for (int v = 0; v < I8_ROWS_WAVES; v++) sum += reinterpret_cast<const int *>(&part[v][(ch >> 2) * 16 + row])[ch & 3];
+        if (row < a.M && n < a.N) ((T *)a.y)[row * a.y_stride + n] = i8_out<T>(sum, xs[row], a.ws[n], (const T *)a.bias, n);
+    }
+}
+
 // ---- many rows: a matrix product ------------------------------------------------------------------------------------------------
 // BM rows x 128 channels per workgroup of four waves (2 x 2, each BM / 2 rows x 64 channels) on v_mfma_i32_32x32x32_i8.  Slices of 128 bytes of K
 // go from memory into LDS without registers (global_load_lds_dwordx4: a wave's instruction brings 128 bytes of each of 8 rows), STAGES of them in
@@ -162,8 +226,8 @@ template <typename T, int BM, int STAGES> __global__ __launch_bounds__(256) void
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
     // Each XCD (workgroup number mod 8) works through a range of tiles of its own in which the channels change fastest within bands of an
     // eighth of all channels: its L2 keeps the band's weights, and a row panel is read once per band.
-    const int total = tiles_m * tiles_n, per = (total + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= per || id >= total) return;
+    const int total = tiles_m * tiles_n * a.splits, per = (total + 7) / 8, all = (blockIdx.x & 7) * per + (blockIdx.x >> 3), split = all % a.splits, id = all / a.splits;
+    if ((int)(blockIdx.x >> 3) >= per || all >= total) return;
     const int band_n = (tiles_n + 7) / 8, band = id / (tiles_m * band_n), in = id - band * tiles_m * band_n;
     const int width = min(band_n, tiles_n - band * band_n), tm = in / width, tn = band * band_n + in - tm * width;
     const int m0 = tm * BM, n0 = tn * I8_BN;
@@ -176,7 +240,7 @@ template <typename T, int BM, int STAGES> __global__ __launch_bounds__(256) void
         const int row = (i * 4 + wave) * 8 + (lane >> 3), p = piece ^ i8_swizzle(row);
         src[i] = i * 32 >= BM ? a.w + (int64_t)min(n0 + row - BM, a.N - 1) * a.w_stride + p * 16 : a.xq + (int64_t)min(m0 + row, a.M - 1) * a.ldq + p * 16;
     }
-    const int slices = a.ldq / I8_BK;
+    const int slices = a.ldq / I8_BK, s_begin = split * slices / a.splits, s_end = (split + 1) * slices / a.splits;
     // loads [from, to) of slice s
     auto issue = [&](int s, int from, int to) {
         const unsigned base = lds_addr(lds) + (s % STAGES) * STAGE;
@@ -191,7 +255,7 @@ template <typename T, int BM, int STAGES> __global__ __launch_bounds__(256) void
     i32x16 acc[NJ][MI] = {};
 #pragma unroll
     for (int s = 0; s < STAGES - 1; s++)
-        if (s < slices) issue(s, 0, LOADS);
+        if (s_begin + s < s_end) issue(s_begin + s, 0, LOADS);
     // scales and bias of the tile, f32 (read one by one behind the loop, they cost four times what the products do)
     float *sw = reinterpret_cast<float *>(lds + i8_tile_lds<T, BM, STAGES>()) - BM - 2 * I8_BN, *sb = sw + I8_BN, *sx = sb + I8_BN;
     if (tid < I8_BN) {
@@ -200,15 +264,15 @@ template <typename T, int BM, int STAGES> __global__ __launch_bounds__(256) void
         sb[tid] = a.bias ? (float)((const T *)a.bias)[n] : 0.f;
     }
     for (int i = tid; i < BM; i += 256) sx[i] = a.xs[min(m0 + i, a.M - 1)];
-    for (int s = 0; s < slices; s++) {
+    for (int s = s_begin; s < s_end; s++) {
         // slice s has landed when at most the younger slices' loads are in flight; behind the barrier everyone's has, and everyone is done with the
         // slice that the next loads overwrite
         // (this wave's own LDS reads of that slice have returned too: the compiler may place the products that use them behind the barrier)
-        if (STAGES == 3 && s + 1 < slices) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
+        if (STAGES == 3 && s + 1 < s_end) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         // The operands of step k + 1 are read, and a quarter of the next loads requested, in front of step k's products.
         const char *buf = lds + (s % STAGES) * STAGE;
-        const bool more = s + STAGES - 1 < slices;
+        const bool more = s + STAGES - 1 < s_end;
         i32x4 wf[2][NJ], xf[2][MI];
         auto read = [&](int k) {
             const int q = k * 2 + (lane >> 5);
@@ -233,6 +297,21 @@ template <typename T, int BM, int STAGES> __global__ __launch_bounds__(256) void
 #pragma unroll
                 for (int i = 0; i < MI; i++) acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[k & 1][j], xf[k & 1][i], acc[j][i], 0, 0, 0);
         }
+    }
+    if (a.splits > 1) {
+        const int64_t ld = (int64_t)tiles_n * I8_BN;
+        int *part = a.part + ((int64_t)split * tiles_m * BM + m0) * ld + n0;
+#pragma unroll
+        for (int i = 0; i < MI; i++)
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const int row = wm * (BM / 2) + i * 32 + (lane & 31), ch = wn * 64 + j * 32 + g * 8 + (lane >> 5) * 4;
+                    const i32x4 v = {acc[j][i][g * 4], acc[j][i][g * 4 + 1], acc[j][i][g * 4 + 2], acc[j][i][g * 4 + 3]};
+                    *reinterpret_cast<i32x4 *>(part + row * ld + ch) = v;
+                }
+        return;
     }
     __syncthreads();
     // lane: row lane % 32 of a block, channels 8 g + 4 (lane / 32) + 0..3 in registers 4 g + 0..3
@@ -269,6 +348,23 @@ template <typename T, int BM, int STAGES> __global__ __launch_bounds__(256) void
             const int row = i / I8_BN, ch = i - row * I8_BN;
             if (ch < cols) y[row * a.y_stride + ch] = out[row * LD + ch];
         }
+    }
+}
+
+
+// Adds the parts (whole numbers: exact in any order) and scales: four channels per thread.
+template <typename T> __global__ __launch_bounds__(256) void k_linear_i8_join(LinearI8Args a, int64_t ld, int64_t step) {
+    const int groups = (a.N + 3) / 4;
+    const int64_t total = (int64_t)a.M * groups;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / groups;
+        const int n = (int)(i - m * groups) * 4;
+        i32x4 sum = *reinterpret_cast<const i32x4 *>(a.part + m * ld + n);
+        for (int s = 1; s < a.splits; s++) sum += *reinterpret_cast<const i32x4 *>(a.part + s * step + m * ld + n);
+        const float xs = a.xs[m];
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (n + r < a.N) ((T *)a.y)[m * a.y_stride + n + r] = i8_out<T>(sum[r], xs, a.ws[n + r], (const T *)a.bias, n + r);
     }
 }
 

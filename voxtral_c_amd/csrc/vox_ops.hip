@@ -301,9 +301,35 @@ template <typename T> void launch_quant(const T *x, int64_t stride, int64_t rows
     if (wide) hipLaunchKernelGGL((k_quant_rows_i8<T, N>), dim3((unsigned)rows), dim3(256), 0, s, x, stride, K, ldq, q, scale);
     else hipLaunchKernelGGL((k_quant_rows_i8<T, 1>), dim3((unsigned)rows), dim3(256), 0, s, x, stride, K, ldq, q, scale);
 }
-template <typename T, int BM, int STAGES> void launch_i8_tile(const LinearI8Args &a, hipStream_t s) {
-    const int tm = (a.M + BM - 1) / BM, tn = (a.N + I8_BN - 1) / I8_BN;
-    hipLaunchKernelGGL((k_linear_i8_tile<T, BM, STAGES>), dim3((unsigned)round_up((int64_t)tm * tn, 8)), dim3(256), (i8_tile_lds<T, BM, STAGES>()), s, a, tm, tn);
+// Up to 32 rows the product is a read of the weights (k_linear_i8_rows).  Above, tiles of 128 rows x 128 channels, of 64 rows where there would be
+// fewer than 192; K is split where even those are fewer than 100, into parts of six slices of 128 or more: the parts' way through memory and
+// the third launch cost 6 - 9 us (64 x 5120 x 1280: 20.7 -> 17.3 us; 256 x 5120 x 5120, 160 tiles: 28.7 us whole, 31.7 split).
+struct I8Plan { bool few; int BM, tiles_m, tiles_n, splits; int64_t scale_at, part_at, ws; };
+I8Plan i8_plan(int64_t rows, int K, int N, bool wide) {
+    I8Plan p{};
+    p.splits = 1;
+    p.few = wide && rows <= I8_FEW_ROWS && rows * K <= I8_FEW;
+    if (p.few) return p;
+    p.scale_at = round_up(rows * i8_ldq(K), 256);
+    p.part_at = p.ws = p.scale_at + round_up(rows * 4, 256);
+    if (!wide || rows <= 32 || N == 0) return p;
+    p.tiles_n = (N + I8_BN - 1) / I8_BN;
+    for (p.BM = 128;; p.BM = 64) {
+        p.tiles_m = (int)((rows + p.BM - 1) / p.BM);
+        if (p.BM == 64 || (int64_t)p.tiles_m * p.tiles_n >= 192) break;
+    }
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+    if (tiles < 100) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(256 / tiles, i8_ldq(K) / I8_BK / 6));
+    if (p.splits > 1) p.ws += (int64_t)p.splits * p.tiles_m * p.BM * p.tiles_n * I8_BN * 4;
+    return p;
+}
+template <typename T, int BM, int STAGES> void launch_i8_tile(const LinearI8Args &a, const I8Plan &p, hipStream_t s) {
+    const int64_t total = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+    hipLaunchKernelGGL((k_linear_i8_tile<T, BM, STAGES>), dim3((unsigned)round_up(total, 8)), dim3(256), (i8_tile_lds<T, BM, STAGES>()), s, a, p.tiles_m, p.tiles_n);
+    if (p.splits > 1) {
+        const int64_t ld = (int64_t)p.tiles_n * I8_BN, groups = (int64_t)a.M * ((a.N + 3) / 4);
+        hipLaunchKernelGGL(k_linear_i8_join<T>, dim3((unsigned)std::min<int64_t>((groups + 255) / 256, 2048)), dim3(256), 0, s, a, ld, ld * p.tiles_m * BM);
+    }
 }
 }  // namespace
 extern "C" int vox_hip_quantize_rows_i8(int dtype, const void *x, int64_t row_stride, int64_t rows, int K, int8_t *q, float *scale, int device, void *stream) {
@@ -322,7 +348,7 @@ extern "C" int vox_hip_quantize_rows_i8(int dtype, const void *x, int64_t row_st
 extern "C" int64_t vox_hip_linear_i8_workspace(int dtype, int64_t rows, int K, int N) {
     if (check_i8("vox_hip_linear_i8", dtype, rows, K)) return -1;
     CHECK(N >= 0 && N <= (1 << 24), "vox_hip_linear_i8: N %d", N);
-    return round_up(rows * i8_ldq(K), 256) + rows * 4;
+    return std::max(i8_plan(rows, K, N, true).ws, i8_plan(rows, K, N, false).ws);         // (w's alignment is not known here)
 }
 extern "C" int vox_hip_linear_i8(int dtype, const void *x, int64_t x_stride, int64_t rows, int K, int N, const int8_t *w, int64_t w_stride, const float *w_scale,
                                  const void *bias, void *y, int64_t y_stride, void *ws, size_t ws_bytes, int device, void *stream) {
@@ -336,21 +362,27 @@ extern "C" int vox_hip_linear_i8(int dtype, const void *x, int64_t x_stride, int
     if (!on.ok) return -1;
     const int ldq = i8_ldq(K);
     int8_t *xq = (int8_t *)ws;
-    float *xs = (float *)((char *)ws + round_up(rows * ldq, 256));
-    LinearI8Args a{xq, xs, w, w_stride, w_scale, bias, y, y_stride, (int)rows, K, N, ldq};
-    const hipStream_t st = (hipStream_t)stream;
     const bool wide = K % 16 == 0 && w_stride % 16 == 0 && aligned(w, 16);
+    const I8Plan p = i8_plan(rows, K, N, wide);
+    float *xs = (float *)((char *)ws + p.scale_at);
+    LinearI8Args a{xq, xs, w, w_stride, w_scale, bias, y, y_stride, (int)rows, K, N, ldq, (int *)((char *)ws + p.part_at), p.splits};
+    const hipStream_t st = (hipStream_t)stream;
     by_type(dtype, [&](auto z) {
         typedef decltype(z) T;
+        if (p.few) {
+            constexpr int V = 16 / sizeof(T);
+            const unsigned lds = (unsigned)(rows * (ldq + 16));
+            if (K % V == 0 && x_stride % V == 0 && aligned(x, 16)) hipLaunchKernelGGL((k_linear_i8_few<T, V>), dim3((N + 15) / 16), dim3(64 * I8_ROWS_WAVES), lds, st, a, (const T *)x, x_stride);
+            else hipLaunchKernelGGL((k_linear_i8_few<T, 1>), dim3((N + 15) / 16), dim3(64 * I8_ROWS_WAVES), lds, st, a, (const T *)x, x_stride);
+            return;
+        }
         launch_quant<T>((const T *)x, x_stride, rows, K, ldq, xq, xs, st);
         const dim3 narrow((N + 15) / 16);
         if (!wide) hipLaunchKernelGGL(k_linear_i8_bytes<T>, dim3((N + 63) / 64, (unsigned)((rows + 63) / 64)), dim3(256), 0, st, a);
         else if (rows <= 16) hipLaunchKernelGGL((k_linear_i8_rows<T, 1>), narrow, dim3(64 * I8_ROWS_WAVES), 0, st, a);
         else if (rows <= 32) hipLaunchKernelGGL((k_linear_i8_rows<T, 2>), narrow, dim3(64 * I8_ROWS_WAVES), 0, st, a);
-        else if (rows <= 64) hipLaunchKernelGGL((k_linear_i8_rows<T, 4>), narrow, dim3(64 * I8_ROWS_WAVES), 0, st, a);
-        else if (0) launch_i8_tile<T, 256, 3>(a, st);
-        else if ((rows + 127) / 128 * ((N + 127) / 128) >= 256) launch_i8_tile<T, 128, 2>(a, st);
-        else launch_i8_tile<T, 64, 3>(a, st);
+        else if (p.BM == 128) launch_i8_tile<T, 128, 2>(a, p, st);
+        else launch_i8_tile<T, 64, 3>(a, p, st);
     });
     return launched("vox_hip_linear_i8");
 }

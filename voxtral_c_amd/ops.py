@@ -79,7 +79,7 @@ def _device(who, *tensors):
     """The tensors' one GPU, as its number."""
     d = tensors[0].get_device()
     for t in tensors:
-        if t.get_device() != d or d < 0 or not t.is_cuda:
+        if t.get_device() != d or d < 0:
             raise ValueError(f"{who}: tensors on {tensors[0].device} and {t.device}: " + ("one device is needed" if t.device != tensors[0].device else
                                                                                             "a GPU is needed (there is no CPU path)"))
     return d
@@ -108,7 +108,7 @@ def tree_plan(parents, n_nodes=None):
         n_nodes = _table(who, "n_nodes", n_nodes, (B,))
     d = _device(who, parents, *(() if n_nodes is None else (n_nodes,)))
     ancestors = parents.new_empty((B, T, (T + 63) // 64), dtype=torch.int64)
-    depth = parents.new_empty((B, T))
+    depth = torch.empty_like(parents)
     if hip.vox_hip_tree_plan(parents.data_ptr(), None if n_nodes is None else n_nodes.data_ptr(), B, T, ancestors.data_ptr(), depth.data_ptr(), d, _stream(d)):
         _error(who)
     return ancestors, depth
@@ -159,7 +159,7 @@ def tree_accept(tokens, choices, root_choice, parents, ancestors, depth, cache_l
     root_choice, cache_len = _table(who, "root_choice", root_choice, (B,)), _table(who, "cache_len", cache_len, (B,))
     ancestors = _table(who, "ancestors", ancestors, (B, T, (T + 63) // 64), torch.int64)
     d = _device(who, tokens, choices, root_choice, parents, ancestors, depth, cache_len)
-    path, n, after, new_len = tokens.new_empty((B, T)), tokens.new_empty((B,)), tokens.new_empty((B,)), tokens.new_empty((B,))
+    path, n, after, new_len = torch.empty_like(tokens), torch.empty_like(root_choice), torch.empty_like(root_choice), torch.empty_like(root_choice)
     if hip.vox_hip_tree_accept(tokens.data_ptr(), choices.data_ptr(), root_choice.data_ptr(), parents.data_ptr(), ancestors.data_ptr(), depth.data_ptr(),
                                cache_len.data_ptr(), B, T, path.data_ptr(), n.data_ptr(), after.data_ptr(), new_len.data_ptr(), d, _stream(d)):
         _error(who)
