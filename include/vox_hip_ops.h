@@ -47,7 +47,7 @@ int vox_hip_tree_plan(const int32_t *parents, const int32_t *n_nodes, int batch,
  *   (position p lives in row p % cap of the ring), and
  *   the nodes j in ancestors[b, i] (any bit set, not only trees') with window <= 0 or depth[j] > depth[i] - window;
  * kv head = h / (heads / kv_heads).  scale is finite and not 0.  A row with depth -1 or with nothing to attend to gives zeros (lse = -inf); what masked keys and
- * values hold, NaN and infinities too, does not matter.  cache_len <= 0 is an empty cache.  Sums and softmax statistics are f32. */
+ * values hold, NaN and infinities too, does not matter (one that a row does see makes the row's outputs infinite or NaN).  cache_len <= 0 is an empty cache.  Sums and softmax statistics are f32. */
 typedef struct vox_hip_tree_attn {
     const void *q, *k, *v;               /* [batch, nodes, heads | kv_heads, head_dim] */
     const void *k_cache, *v_cache;       /* [batch, cap, kv_heads, head_dim] */

@@ -210,6 +210,16 @@ def test_tree_attention_passes_on_what_is_seen(dtype, H):
     assert torch.equal(torch.nan_to_num(out, nan=1e9, posinf=2e9, neginf=-2e9), torch.nan_to_num(want, nan=1e9, posinf=2e9, neginf=-2e9))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("H", [2, 4, 40])
+def test_tree_attention_depths_of_ones_own(dtype, H):
+    """Depths that no tree of this size has (nodes far behind the cache's end): windows that lie inside, at the end of, and behind the cache."""
+    c = attn_case(17, dtype, 2, 5, H, 2, 64, 300, [290, 120], shorter=False)
+    c["depth"] = dev(np.array([[0, 150, 199, 200, 2 ** 31 - 1], [3, 60, 119, 1, -1]], np.int32))
+    check_attn(c, window=200)
+    check_attn(c, window=1)
+
+
 def test_tree_attention_scale():
     c = attn_case(14, F32, 1, 5, 4, 2, 64, 40, [33])
     check_attn(c, scale=-0.2)

@@ -88,7 +88,7 @@ def test_tree_commit_refuses():
 def test_token_scores_refuses():
     x, t = zeros(4, 100), zeros(4, 2, dtype=I32)
     for args, message in (((x[0], t), "rows, vocab"), ((x.double(), t), "float32"), ((x, t.long()), "tokens"), ((x, t[:3]), "tokens"), ((x, t, 65), "top"), ((x, t, -1), "top"),
-                          ((x[:, :10].contiguous(), t, 11), "top"), ((x.t(), zeros(100, 2, dtype=I32)), "not contiguous"), ((zeros(4, 0), None), "rows, vocab"), ((x, t, 3), "GPU")):
+                          ((x[:, :10].contiguous(), t, 11), "top"), ((x.t(), zeros(100, 2, dtype=I32)), "not contiguous"), ((zeros(4, 0), None), "rows, vocab"), ((x, t[0, 0]), "tokens"), ((x, t[None]), "tokens"), ((x, t, 3), "GPU")):
         with pytest.raises(ValueError, match=message):
             ops.token_scores(*args)
 
@@ -136,6 +136,8 @@ def test_c_entries_refuse_before_any_launch():
     assert need > 0 and lin(fake, need - 1) == -1 and "workspace" in err()
     assert lin(fake, need, 6) == -1 and "strides" in err()
     assert v.hip.vox_hip_linear_i8_workspace(0, 3, 131073, 7) == -1 and "131072" in err()
+    assert v.hip.vox_hip_linear_i8_workspace(0, 4194241, 64, 7) == -1 and "rows" in err()
+    assert v.hip.vox_hip_linear_i8_workspace(0, 4194240, 64, 1 << 24) == -1 and "N" in err()
     assert v.hip.vox_hip_quantize_rows_i8(0, None, 8, 2, 8, fake, fake, 0, None) == -1 and "null" in err()
     if v.device_count() == 0:
         assert v.hip.vox_hip_tree_plan(fake, None, 1, 4, fake, fake, 0, None) == -1 and "no such device" in err()

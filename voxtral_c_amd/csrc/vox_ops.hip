@@ -288,9 +288,10 @@ extern "C" int vox_hip_token_scores(int dtype, const void *logits, int64_t row_s
 
 // ---- 8-bit integers ----------------------------------------------------------------------------------------------------------
 namespace {
+constexpr int I8_MAX_ROWS = 65535 * 64;                      // (a grid's second dimension)
 int check_i8(const char *who, int dtype, int64_t rows, int K) {
     CHECK(dtype_size(dtype), "%s: dtype %d", who, dtype);
-    CHECK(rows >= 0 && rows <= (1 << 22), "%s: %lld rows (at most %d)", who, (long long)rows, 1 << 22);
+    CHECK(rows >= 0 && rows <= I8_MAX_ROWS, "%s: %lld rows (at most %d)", who, (long long)rows, I8_MAX_ROWS);
     CHECK(K >= 1 && K <= VOX_I8_MAX_K, "%s: K %d (1 to %d)", who, K, VOX_I8_MAX_K);
     return 0;
 }
@@ -347,7 +348,7 @@ extern "C" int vox_hip_quantize_rows_i8(int dtype, const void *x, int64_t row_st
 }
 extern "C" int64_t vox_hip_linear_i8_workspace(int dtype, int64_t rows, int K, int N) {
     if (check_i8("vox_hip_linear_i8", dtype, rows, K)) return -1;
-    CHECK(N >= 0 && N <= (1 << 24), "vox_hip_linear_i8: N %d", N);
+    CHECK(N >= 0 && N <= (1 << 24) && (rows / 64 + 1) * (N / 128 + 1) < ((int64_t)1 << 30), "vox_hip_linear_i8: N %d, %lld rows", N, (long long)rows);
     return std::max(i8_plan(rows, K, N, true).ws, i8_plan(rows, K, N, false).ws);         // (w's alignment is not known here)
 }
 extern "C" int vox_hip_linear_i8(int dtype, const void *x, int64_t x_stride, int64_t rows, int K, int N, const int8_t *w, int64_t w_stride, const float *w_scale,

@@ -260,7 +260,7 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, (DP == 256 || (ATTN_SPLIT<T, SHARE
     for (int t = 0; t < RT; t++) {
         const int row = wrow0 + t * 16 + n16, node = row < R ? row / a.G : 0, h = kvh * a.G + (row - node * a.G);
         row_node[t] = node;
-        row_depth[t] = row < R ? a.depth[(size_t)b * a.T + node] : -1;
+        row_depth[t] = row < R ? min(a.depth[(size_t)b * a.T + node], 1 << 30) : -1;
         const T *q = (const T *)a.q + b * a.q_sb + node * a.q_st + h * a.q_sh;
         auto load = [&](int d) {
             kvec x = kvec(T(0.f));
@@ -286,10 +286,24 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, (DP == 256 || (ATTN_SPLIT<T, SHARE
         const unsigned slot = slot_first + (unsigned)t * KT;
         return slot >= (unsigned)a.cap ? slot - a.cap : slot;
     };
-    // Tiles [full_begin, full_end) are seen whole by every row: behind the window's edge of the deepest node, in front of the cache's end.  A tile of
+    // Tiles [full_begin, full_end) are seen whole by every row of the workgroup: behind the window's edge of its deepest one, in front of the cache's
+    // end.  A tile of
     // those that the ring does not break is plain: its rows follow each other, and a lane's offsets within it are the same for every tile.
     const int edge = (int)max(tr.len + 1 - a.window - tr.first, (int64_t)-(1 << 30));            // first position of a window at depth 0, from `first`
-    const int full_begin = a.window > 0 && edge + a.T > 0 ? (edge + a.T - 1) / KT + 1 : 0, full_end = tr.cached / KT;
+    int deepest = 0;
+    if (a.window > 0) {                                      // (of this workgroup's rows: the deepest node's window begins last)
+        __shared__ int depths[RW];
+#pragma unroll
+        for (int r = 0; r < RT; r++) deepest = max(deepest, row_depth[r]);
+#pragma unroll
+        for (int i = 1; i < 16; i <<= 1) deepest = max(deepest, __shfl_xor(deepest, i, 64));
+        if (lane == 0) depths[rw] = deepest;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < RW; i++) deepest = max(deepest, depths[i]);
+        deepest = __builtin_amdgcn_readfirstlane(deepest);
+    }
+    const int full_begin = a.window > 0 && edge + deepest > 0 ? (edge + deepest - 1) / KT + 1 : 0, full_end = tr.cached / KT;
     auto is_masked = [&](int t) { return t < full_begin || t >= full_end; };
     auto is_plain = [&](int t) { return a.D == DP && t < full_end && slot_of(t) + KT <= (unsigned)a.cap; };
     auto tile_at = [&](int t) {

@@ -207,7 +207,7 @@ def token_scores(logits, tokens=None, top=0):
         raise ValueError(f"{who}: top {top} of {V} (at most {MAX_TOP})")
     shape = (R, 0)
     if tokens is not None:
-        shape = (R,) if tokens.dim() == 1 else (R, tokens.shape[-1])
+        shape = (R, tokens.shape[1]) if tokens.dim() == 2 else (R,)
         tokens = _table(who, "tokens", tokens, shape)
     d = _device(who, logits) if tokens is None else _device(who, logits, tokens)
     new, f32 = logits.new_empty, torch.float32
