@@ -47,7 +47,7 @@ int vox_hip_tree_plan(const int32_t *parents, const int32_t *n_nodes, int batch,
  *   (position p lives in row p % cap of the ring), and
  *   the nodes j in ancestors[b, i] (any bit set, not only trees') with window <= 0 or depth[j] > depth[i] - window;
  * kv head = h / (heads / kv_heads).  scale is finite and not 0.  A row with depth -1 or with nothing to attend to gives zeros (lse = -inf); what masked keys and
- * values hold, NaN and infinities too, does not matter (one that a row does see makes the row's outputs infinite or NaN).  cache_len <= 0 is an empty cache.  Sums and softmax statistics are f32. */
+ * values hold, NaN and infinities too, does not matter (one that a row does see may make the row's outputs infinite or NaN).  cache_len <= 0 is an empty cache.  Sums and softmax statistics are f32. */
 typedef struct vox_hip_tree_attn {
     const void *q, *k, *v;               /* [batch, nodes, heads | kv_heads, head_dim] */
     const void *k_cache, *v_cache;       /* [batch, cap, kv_heads, head_dim] */
@@ -84,7 +84,8 @@ int vox_hip_tree_commit(int dtype, int layers, int batch, int nodes, int kv_head
  * logprob [rows, given] of tokens [rows, given] (contiguous; an id outside the vocabulary gives -inf), entropy [rows] in nats, lse [rows],
  * the `top` largest logits' indexes and log probabilities [rows, top], equal logits by the lowest index.  given = 0 / top = 0: those
  * pointers may be NULL.  A logit of -inf is a token of probability 0 (a row of nothing else: lse -inf, entropy 0, every logprob -inf);
- * a NaN makes its row's lse, entropy and logprobs NaN and counts as the largest; +inf makes lse +inf and the probabilities NaN. */
+ * a NaN makes its row's lse, entropy and logprobs NaN and counts as the largest; +inf without a NaN makes lse +inf and
+ * the entropy and log probabilities NaN. */
 int64_t vox_hip_token_scores_workspace(int dtype, int64_t rows, int vocab, int top);
 int vox_hip_token_scores(int dtype, const void *logits, int64_t row_stride, int64_t rows, int vocab, const int32_t *tokens, int given, int top,
                          float *logprob, float *entropy, float *lse, int32_t *top_index, float *top_logprob, void *ws, size_t ws_bytes,

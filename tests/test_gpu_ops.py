@@ -374,6 +374,26 @@ def test_token_scores_switched_off_and_broken_rows():
     check_scores(x[:3], t[:3], 12)                                     # their neighbours are as before
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [70, 9001, 131072])
+def test_token_scores_infinity_and_nan_in_one_row(dtype, V):
+    """A NaN makes its row NaN wherever an infinity stands; without one, the infinity is the log-sum."""
+    rng = np.random.default_rng(33)
+    x = randn(rng, 9, V)
+    x[:, 5] = math.inf
+    at = [0, 4, 6, 33, V // 2, V - 1]
+    for row, i in enumerate(at):
+        x[row, i] = math.nan
+    x[6, V - 2] = math.inf
+    x[7, 6] = -math.inf
+    for top in (0, 3):
+        g = ops.token_scores(x.to(dtype), dev(np.full((9, 1), 7, np.int32)), top)
+        assert torch.isnan(g.lse[:6]).all() and (g.lse[6:] == math.inf).all()
+        assert torch.isnan(g.entropy).all() and torch.isnan(g.logprob).all()
+        if top:
+            assert g.top_index[:6, 0].tolist() == at and (g.top_index[:6, 1] == 5).all() and (g.top_index[6:, 0] == 5).all() and g.top_index[6, 1] == V - 2
+
+
 def test_token_scores_confident_rows_keep_their_digits():
     """One token with almost all the probability: entropy and logprob are small numbers with all their digits, not differences of large ones."""
     x = torch.full((4, 4096), 0.0, device=DEV)

@@ -100,6 +100,8 @@ def test_linear_i8_refuses():
                           ((zeros(1, 131073), zeros(1, 131073, dtype=torch.int8), s[:1]), "131072"), ((x, w, s), "GPU")):
         with pytest.raises(ValueError, match=message):
             ops.linear_i8(*args)
+    with pytest.raises(ValueError, match="gradients"):
+        ops.linear_i8(x, w, s.requires_grad_())
     for x, message in ((zeros(3), "rows, K"), (zeros(3, 0), "rows, K"), (zeros(2, 3, dtype=torch.int32), "float32"), (zeros(2, 3), "GPU")):
         with pytest.raises(ValueError, match=message):
             ops.quantize_rows_i8(x)
@@ -139,5 +141,10 @@ def test_c_entries_refuse_before_any_launch():
     assert v.hip.vox_hip_linear_i8_workspace(0, 4194241, 64, 7) == -1 and "rows" in err()
     assert v.hip.vox_hip_linear_i8_workspace(0, 4194240, 64, 1 << 24) == -1 and "N" in err()
     assert v.hip.vox_hip_quantize_rows_i8(0, None, 8, 2, 8, fake, fake, 0, None) == -1 and "null" in err()
+    far = 1 << 24                                                      # (a grid's threads are counted in 32 bits)
+    assert v.hip.vox_hip_tree_plan(fake, None, far, 1, fake, fake, 0, None) == -1 and "batch" in err()
+    assert v.hip.vox_hip_tree_accept(*[fake] * 7, far, 1, *[fake] * 4, 0, None) == -1 and "batch" in err()
+    assert v.hip.vox_hip_tree_commit(0, 1, far, 1, 1, 8, 9, fake, st, fake, st, fake, st, fake, st, fake, fake, fake, 0, None) == -1 and "batch" in err()
+    assert v.hip.vox_hip_token_scores_workspace(0, far, 1, 0) == -1 and "rows" in err()
     if v.device_count() == 0:
         assert v.hip.vox_hip_tree_plan(fake, None, 1, 4, fake, fake, 0, None) == -1 and "no such device" in err()

@@ -56,6 +56,7 @@ int launched(const char *who) {
     return e == hipSuccess ? 0 : refuse("%s: launch failed: %s", who, hipGetErrorString(e));
 }
 
+constexpr int64_t GRID_MAX = ((int64_t)1 << 24) - 1;         // workgroups of 256 along a grid's first dimension (its threads are counted in 32 bits)
 int dtype_size(int dtype) { return dtype == VOX_F32 ? 4 : dtype == VOX_BF16 || dtype == VOX_F16 ? 2 : 0; }
 bool aligned(const void *p, int64_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
@@ -71,7 +72,7 @@ template <typename F> void by_type(int dtype, F f) {
 // ---- draft trees -------------------------------------------------------------------------------------------------------------
 extern "C" int vox_hip_tree_plan(const int32_t *parents, const int32_t *n_nodes, int batch, int nodes, uint64_t *ancestors, int32_t *depth,
                                  int device, void *stream) {
-    CHECK(batch >= 0 && nodes >= 0 && nodes <= VOX_TREE_MAX_NODES, "vox_hip_tree_plan: batch %d, nodes %d (at most %d nodes)", batch, nodes, VOX_TREE_MAX_NODES);
+    CHECK(batch >= 0 && batch <= GRID_MAX && nodes >= 0 && nodes <= VOX_TREE_MAX_NODES, "vox_hip_tree_plan: batch %d, nodes %d (at most %d nodes)", batch, nodes, VOX_TREE_MAX_NODES);
     if (batch == 0 || nodes == 0) return 0;
     CHECK(parents && ancestors && depth, "vox_hip_tree_plan: null pointer");
     OnDevice on("vox_hip_tree_plan", device);
@@ -83,7 +84,7 @@ extern "C" int vox_hip_tree_plan(const int32_t *parents, const int32_t *n_nodes,
 extern "C" int vox_hip_tree_accept(const int32_t *tokens, const int32_t *choices, const int32_t *root_choice, const int32_t *parents,
                                    const uint64_t *ancestors, const int32_t *depth, const int32_t *cache_len, int batch, int nodes, int32_t *path,
                                    int32_t *n_accepted, int32_t *next_token, int32_t *new_len, int device, void *stream) {
-    CHECK(batch >= 0 && nodes >= 1 && nodes <= VOX_TREE_MAX_NODES, "vox_hip_tree_accept: batch %d, nodes %d (1 to %d nodes)", batch, nodes, VOX_TREE_MAX_NODES);
+    CHECK(batch >= 0 && batch <= GRID_MAX && nodes >= 1 && nodes <= VOX_TREE_MAX_NODES, "vox_hip_tree_accept: batch %d, nodes %d (1 to %d nodes)", batch, nodes, VOX_TREE_MAX_NODES);
     if (batch == 0) return 0;
     CHECK(tokens && choices && root_choice && parents && ancestors && depth && cache_len && path && n_accepted && next_token && new_len,
           "vox_hip_tree_accept: null pointer");
@@ -100,7 +101,7 @@ extern "C" int vox_hip_tree_commit(int dtype, int layers, int batch, int nodes, 
                                    int device, void *stream) {
     const int size = dtype_size(dtype);
     CHECK(size, "vox_hip_tree_commit: dtype %d", dtype);
-    CHECK(layers >= 0 && layers <= 32767 && batch >= 0 && nodes >= 0 && nodes <= VOX_TREE_MAX_NODES && kv_heads >= 1 && kv_heads <= 4096 && head_dim >= 1 && head_dim <= 4096,
+    CHECK(layers >= 0 && layers <= 32767 && batch >= 0 && batch <= GRID_MAX && nodes >= 0 && nodes <= VOX_TREE_MAX_NODES && kv_heads >= 1 && kv_heads <= 4096 && head_dim >= 1 && head_dim <= 4096,
           "vox_hip_tree_commit: layers %d, batch %d, nodes %d, kv_heads %d, head_dim %d", layers, batch, nodes, kv_heads, head_dim);
     if (layers == 0 || batch == 0 || nodes == 0) return 0;
     CHECK(cap >= nodes, "vox_hip_tree_commit: a ring of %d rows does not hold a path of %d nodes", cap, nodes);
@@ -251,7 +252,7 @@ ScorePlan score_plan(int64_t rows, int vocab, int top) {
 }
 int check_scores(int dtype, int64_t rows, int vocab, int top) {
     CHECK(dtype_size(dtype), "vox_hip_token_scores: dtype %d", dtype);
-    CHECK(rows >= 0 && rows <= (1 << 26), "vox_hip_token_scores: %lld rows", (long long)rows);
+    CHECK(rows >= 0 && rows <= GRID_MAX, "vox_hip_token_scores: %lld rows (at most %lld)", (long long)rows, (long long)GRID_MAX);
     CHECK(vocab >= 1 && vocab <= (1 << 30), "vox_hip_token_scores: a vocabulary of %d", vocab);
     CHECK(top >= 0 && top <= VOX_SCORES_MAX_TOP && top <= vocab, "vox_hip_token_scores: top %d of %d (at most %d)", top, vocab, VOX_SCORES_MAX_TOP);
     return 0;
@@ -348,7 +349,7 @@ extern "C" int vox_hip_quantize_rows_i8(int dtype, const void *x, int64_t row_st
 }
 extern "C" int64_t vox_hip_linear_i8_workspace(int dtype, int64_t rows, int K, int N) {
     if (check_i8("vox_hip_linear_i8", dtype, rows, K)) return -1;
-    CHECK(N >= 0 && N <= (1 << 24) && (rows / 64 + 1) * (N / 128 + 1) < ((int64_t)1 << 30), "vox_hip_linear_i8: N %d, %lld rows", N, (long long)rows);
+    CHECK(N >= 0 && N <= (1 << 24) && (rows / 64 + 1) * (N / 128 + 1) <= GRID_MAX / 8, "vox_hip_linear_i8: N %d, %lld rows", N, (long long)rows);
     return std::max(i8_plan(rows, K, N, true).ws, i8_plan(rows, K, N, false).ws);         // (w's alignment is not known here)
 }
 extern "C" int vox_hip_linear_i8(int dtype, const void *x, int64_t x_stride, int64_t rows, int K, int N, const int8_t *w, int64_t w_stride, const float *w_scale,

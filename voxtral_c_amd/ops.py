@@ -248,6 +248,8 @@ def linear_i8(x, w, w_scale, bias=None):
     if w.dtype != torch.int8 or w.shape[1] != K or (w.stride(1) != 1 and K > 1):
         raise ValueError(f"{who}: w is {w.dtype} {tuple(w.shape)}: int8 {(N, K)} with contiguous rows is needed")
     w_scale = _table(who, "w_scale", w_scale, (N,), torch.float32)
+    if w_scale.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{who}: w_scale needs gradients: there is no backward pass (use torch.no_grad())")
     d = _device(who, x, w, w_scale, *(() if bias is None else (bias,)))
     y = x.new_empty((M, N))
     need = hip.vox_hip_linear_i8_workspace(number, M, K, N)
