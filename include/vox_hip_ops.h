@@ -98,7 +98,7 @@ int vox_hip_quantize_rows_i8(int dtype, const void *x, int64_t row_stride, int64
 /* y[m, n] = x_scale[m] * w_scale[n] * sum_k xq[m, k] * w[n, k] (+ bias[n]): x [rows, K] is quantised as above within the call, the sum is
  * exact.  w [N, K] int8 (row stride in bytes), w_scale [N] f32, bias [N] in x's type or NULL, y [rows, N] in x's type,
  * row stride in elements. */
-int64_t vox_hip_linear_i8_workspace(int dtype, int64_t rows, int K, int N);
+int64_t vox_hip_linear_i8_workspace(int dtype, int64_t rows, int K, int N, const int8_t *w, int64_t w_stride);      /* (reads w's alignment) */
 int vox_hip_linear_i8(int dtype, const void *x, int64_t x_stride, int64_t rows, int K, int N, const int8_t *w, int64_t w_stride,
                       const float *w_scale, const void *bias, void *y, int64_t y_stride, void *ws, size_t ws_bytes, int device, void *stream);
 

@@ -133,13 +133,13 @@ def test_c_entries_refuse_before_any_launch():
     score = lambda ws, n: v.hip.vox_hip_token_scores(0, fake, 131072, 1, 131072, fake, 1, 8, fake, fake, fake, fake, fake, ws, n, 0, None)  # noqa: E731
     for ws, n in ((None, 0), (fake, need - 1), (fake + 16, need)):
         assert score(ws, n) == -1 and "workspace" in err()
-    need = v.hip.vox_hip_linear_i8_workspace(0, 3, 100, 7)
+    need = v.hip.vox_hip_linear_i8_workspace(0, 3, 100, 7, fake, 100)
     lin = lambda ws, n, ys=7: v.hip.vox_hip_linear_i8(0, fake, 100, 3, 100, 7, fake, 100, fake, None, fake, ys, ws, n, 0, None)  # noqa: E731
     assert need > 0 and lin(fake, need - 1) == -1 and "workspace" in err()
     assert lin(fake, need, 6) == -1 and "strides" in err()
-    assert v.hip.vox_hip_linear_i8_workspace(0, 3, 131073, 7) == -1 and "131072" in err()
-    assert v.hip.vox_hip_linear_i8_workspace(0, 4194241, 64, 7) == -1 and "rows" in err()
-    assert v.hip.vox_hip_linear_i8_workspace(0, 4194240, 64, 1 << 24) == -1 and "N" in err()
+    assert v.hip.vox_hip_linear_i8_workspace(0, 3, 131073, 7, fake, 131073) == -1 and "131072" in err()
+    assert v.hip.vox_hip_linear_i8_workspace(0, 4194241, 64, 7, fake, 64) == -1 and "rows" in err()
+    assert v.hip.vox_hip_linear_i8_workspace(0, 4194240, 64, 1 << 24, fake, 64) == -1 and "N" in err()
     assert v.hip.vox_hip_quantize_rows_i8(0, None, 8, 2, 8, fake, fake, 0, None) == -1 and "null" in err()
     far = 1 << 24                                                      # (a grid's threads are counted in 32 bits)
     assert v.hip.vox_hip_tree_plan(fake, None, far, 1, fake, fake, 0, None) == -1 and "batch" in err()

@@ -29,13 +29,15 @@ __device__ __forceinline__ RowScale row_scale(unsigned amax_bits) {
 
 // One workgroup per row: q [rows, ldq] (columns K .. ldq - 1 are zeros), scale [rows].  Bound by the row's two trips (the second one hits the
 // caches; keeping the row in registers instead measured the same).  N elements per load: K, stride and x allow it, and ldq % N = 0.
-template <typename T, int N> __global__ __launch_bounds__(256) void k_quant_rows_i8(const T *x, int64_t stride, int K, int ldq, int8_t *q, float *scale) {
-    __shared__ unsigned red[4];
+constexpr int I8_QUANT_THREADS = 1024;
+template <typename T, int N> __global__ __launch_bounds__(I8_QUANT_THREADS) void k_quant_rows_i8(const T *x, int64_t stride, int K, int ldq, int8_t *q, float *scale) {
+    __shared__ unsigned red[I8_QUANT_THREADS / 64];
     const int64_t row = blockIdx.x;
+    const int threads = blockDim.x;
     const T *xr = x + row * stride;
     int8_t *qr = q + row * ldq;
     unsigned m = 0;
-    for (int k = threadIdx.x * N; k < K; k += 256 * N) {
+    for (int k = threadIdx.x * N; k < K; k += threads * N) {
         float v[N];
         load_vec<T, N>(v, xr + k);
 #pragma unroll
@@ -44,8 +46,10 @@ template <typename T, int N> __global__ __launch_bounds__(256) void k_quant_rows
     m = wave_max_u(m);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
     __syncthreads();
-    const RowScale r = row_scale(max(max(red[0], red[1]), max(red[2], red[3])));
-    for (int k = threadIdx.x * N; k < ldq; k += 256 * N) {
+    m = red[0];
+    for (int w = 1; w < threads >> 6; w++) m = max(m, red[w]);
+    const RowScale r = row_scale(m);
+    for (int k = threadIdx.x * N; k < ldq; k += threads * N) {
         typedef int8_t out __attribute__((ext_vector_type(N)));
         float v[N] = {};
         out o;
@@ -116,11 +120,16 @@ constexpr int I8_ROWS_WAVES = 8;
 template <typename T, int MT> __global__ __launch_bounds__(64 * I8_ROWS_WAVES) void k_linear_i8_rows(LinearI8Args a) {
     __shared__ i32x4 part[I8_ROWS_WAVES][MT][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n16 = lane & 15, c = lane >> 4;
+    static_assert(MT * 256 <= 64 * I8_ROWS_WAVES, "");
     const int n0 = blockIdx.x * 16;
     const int8_t *w = a.w + (int64_t)min(n0 + n16, a.N - 1) * a.w_stride + c * 16;
     const int8_t *x[MT];
 #pragma unroll
     for (int t = 0; t < MT; t++) x[t] = a.xq + (int64_t)min(t * 16 + n16, a.M - 1) * a.ldq + c * 16;
+    // this thread's output, its scales requested in front of the products
+    const int ch = tid & 15, row = tid >> 4, n = n0 + ch;    // (the workgroup has a thread per output or more)
+    const bool mine = tid < MT * 256 && row < a.M && n < a.N;
+    const float out_xs = mine ? a.xs[row] : 0.f, out_ws = mine ? a.ws[n] : 0.f, out_bias = mine && a.bias ? (float)((const T *)a.bias)[n] : 0.f;
     i32x4 acc[MT] = {};
     for (int k = wave * 128; k < a.K; k += 128 * I8_ROWS_WAVES) {
         // (xq holds zeros from K to ldq, a multiple of 128: what stands in for weights behind K does not matter, so it is the row's first bytes)
@@ -135,14 +144,12 @@ template <typename T, int MT> __global__ __launch_bounds__(64 * I8_ROWS_WAVES) v
 #pragma unroll
     for (int t = 0; t < MT; t++) part[wave][t][lane] = acc[t];
     __syncthreads();
-    for (int i = tid; i < MT * 256; i += 64 * I8_ROWS_WAVES) {
-        // channel i % 16 of row i / 16: element (channel % 4) of lane (channel / 4) * 16 + row % 16
-        const int ch = i & 15, row = i >> 4, n = n0 + ch;
-        int sum = 0;
+    if (!mine) return;
+    // channel ch of row: element (ch % 4) of lane (ch / 4) * 16 + row % 16
+    int sum = 0;
 #pragma unroll
-        for (int v = 0; v < I8_ROWS_WAVES; v++) sum += reinterpret_cast<const int *>(&part[v][row >> 4][(ch >> 2) * 16 + (row & 15)])[ch & 3];
-        if (row < a.M && n < a.N) ((T *)a.y)[row * a.y_stride + n] = i8_out<T>(sum, a.xs[row], a.ws[n], (const T *)a.bias, n);
-    }
+    for (int v = 0; v < I8_ROWS_WAVES; v++) sum += reinterpret_cast<const int *>(&part[v][row >> 4][(ch >> 2) * 16 + (row & 15)])[ch & 3];
+    ((T *)a.y)[row * a.y_stride + n] = from_f32<T>(i8_scaled(sum, out_xs, out_ws) + out_bias);
 }
 
 // The same in one launch for a few rows (single tokens): every workgroup quantises all of x into its LDS while its first weights are on their way.  Up
@@ -156,6 +163,9 @@ template <typename T, int N> __global__ __launch_bounds__(64 * I8_ROWS_WAVES) vo
     const int n0 = blockIdx.x * 16, ld = a.ldq + 16;
     const int8_t *w = a.w + (int64_t)min(n0 + n16, a.N - 1) * a.w_stride + c * 16;
     auto weights = [&](int k) { return *reinterpret_cast<const i32x4 *>(w + (k + c * 16 < a.K ? k : -c * 16)); };       // (see above)
+    const int ch = tid & 15, out_row = tid >> 4, n = n0 + ch;          // this thread's output, its scale requested here
+    const bool mine = tid < 256 && out_row < a.M && n < a.N;
+    const float out_ws = mine ? a.ws[n] : 0.f, out_bias = mine && a.bias ? (float)((const T *)a.bias)[n] : 0.f;
     i32x4 ahead[I8_FEW_AHEAD][2];
 #pragma unroll
     for (int i = 0; i < I8_FEW_AHEAD; i++) {
@@ -198,13 +208,11 @@ template <typename T, int N> __global__ __launch_bounds__(64 * I8_ROWS_WAVES) vo
     for (int k = (wave + I8_FEW_AHEAD * I8_ROWS_WAVES) * 128; k < a.K; k += 128 * I8_ROWS_WAVES) step(k, weights(k), weights(k + 64));
     part[wave][lane] = acc;
     __syncthreads();
-    if (tid < 256) {
-        const int ch = tid & 15, row = tid >> 4, n = n0 + ch;
-        int sum = 0;
+    if (!mine) return;
+    int sum = 0;
 #pragma unroll
-        for (int v = 0; v < I8_ROWS_WAVES; v++) sum += reinterpret_cast<const int *>(&part[v][(ch >> 2) * 16 + row])[ch & 3];
-        if (row < a.M && n < a.N) ((T *)a.y)[row * a.y_stride + n] = i8_out<T>(sum, xs[row], a.ws[n], (const T *)a.bias, n);
-    }
+    for (int v = 0; v < I8_ROWS_WAVES; v++) sum += reinterpret_cast<const int *>(&part[v][(ch >> 2) * 16 + out_row])[ch & 3];
+    ((T *)a.y)[out_row * a.y_stride + n] = from_f32<T>(i8_scaled(sum, xs[out_row], out_ws) + out_bias);
 }
 
 // ---- many rows: a matrix product ------------------------------------------------------------------------------------------------

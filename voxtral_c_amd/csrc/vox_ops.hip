@@ -289,7 +289,7 @@ extern "C" int vox_hip_token_scores(int dtype, const void *logits, int64_t row_s
 
 // ---- 8-bit integers ----------------------------------------------------------------------------------------------------------
 namespace {
-constexpr int I8_MAX_ROWS = 65535 * 64;                      // (a grid's second dimension)
+constexpr int I8_MAX_ROWS = 65535 * 64;                      // (a grid's second dimension; and 2^32 threads of the quantiser's)
 int check_i8(const char *who, int dtype, int64_t rows, int K) {
     CHECK(dtype_size(dtype), "%s: dtype %d", who, dtype);
     CHECK(rows >= 0 && rows <= I8_MAX_ROWS, "%s: %lld rows (at most %d)", who, (long long)rows, I8_MAX_ROWS);
@@ -300,8 +300,9 @@ int i8_ldq(int K) { return (int)round_up(K, I8_BK); }
 template <typename T> void launch_quant(const T *x, int64_t stride, int64_t rows, int K, int ldq, int8_t *q, float *scale, hipStream_t s) {
     constexpr int N = 16 / sizeof(T);
     const bool wide = K % N == 0 && ldq % N == 0 && stride % N == 0 && aligned(x, 16) && aligned(q, 8);
-    if (wide) hipLaunchKernelGGL((k_quant_rows_i8<T, N>), dim3((unsigned)rows), dim3(256), 0, s, x, stride, K, ldq, q, scale);
-    else hipLaunchKernelGGL((k_quant_rows_i8<T, 1>), dim3((unsigned)rows), dim3(256), 0, s, x, stride, K, ldq, q, scale);
+    const int threads = (int)std::min<int64_t>(round_up((ldq + (wide ? N : 1) - 1) / (wide ? N : 1), 64), I8_QUANT_THREADS);      // one load per thread where that is enough
+    if (wide) hipLaunchKernelGGL((k_quant_rows_i8<T, N>), dim3((unsigned)rows), dim3(threads), 0, s, x, stride, K, ldq, q, scale);
+    else hipLaunchKernelGGL((k_quant_rows_i8<T, 1>), dim3((unsigned)rows), dim3(threads), 0, s, x, stride, K, ldq, q, scale);
 }
 // Up to 32 rows the product is a read of the weights (k_linear_i8_rows).  Above, tiles of 128 rows x 128 channels, of 64 rows where there would be
 // fewer than 192; K is split where even those are fewer than 100, into parts of six slices of 128 or more: the parts' way through memory and
@@ -347,24 +348,27 @@ extern "C" int vox_hip_quantize_rows_i8(int dtype, const void *x, int64_t row_st
     });
     return launched("vox_hip_quantize_rows_i8");
 }
-extern "C" int64_t vox_hip_linear_i8_workspace(int dtype, int64_t rows, int K, int N) {
+namespace {
+bool i8_wide(int K, const int8_t *w, int64_t w_stride) { return K % 16 == 0 && w_stride % 16 == 0 && aligned(w, 16); }
+}  // namespace
+extern "C" int64_t vox_hip_linear_i8_workspace(int dtype, int64_t rows, int K, int N, const int8_t *w, int64_t w_stride) {
     if (check_i8("vox_hip_linear_i8", dtype, rows, K)) return -1;
     CHECK(N >= 0 && N <= (1 << 24) && (rows / 64 + 1) * (N / 128 + 1) <= GRID_MAX / 8, "vox_hip_linear_i8: N %d, %lld rows", N, (long long)rows);
-    return std::max(i8_plan(rows, K, N, true).ws, i8_plan(rows, K, N, false).ws);         // (w's alignment is not known here)
+    return i8_plan(rows, K, N, i8_wide(K, w, w_stride)).ws;
 }
 extern "C" int vox_hip_linear_i8(int dtype, const void *x, int64_t x_stride, int64_t rows, int K, int N, const int8_t *w, int64_t w_stride, const float *w_scale,
                                  const void *bias, void *y, int64_t y_stride, void *ws, size_t ws_bytes, int device, void *stream) {
-    const int64_t need = vox_hip_linear_i8_workspace(dtype, rows, K, N);
+    const int64_t need = vox_hip_linear_i8_workspace(dtype, rows, K, N, w, w_stride);
     if (need < 0) return -1;
     CHECK(x_stride >= 0 && w_stride >= 0 && (y_stride >= N || rows <= 1), "vox_hip_linear_i8: strides %lld, %lld, %lld", (long long)x_stride, (long long)w_stride, (long long)y_stride);
     if (rows == 0 || N == 0) return 0;
     CHECK(x && w && w_scale && y, "vox_hip_linear_i8: null pointer");
-    CHECK(ws && aligned(ws, 256) && ws_bytes >= (size_t)need, "vox_hip_linear_i8: needs %lld bytes of workspace, 256-byte aligned", (long long)need);
+    CHECK(need == 0 || (ws && aligned(ws, 256) && ws_bytes >= (size_t)need), "vox_hip_linear_i8: needs %lld bytes of workspace, 256-byte aligned", (long long)need);
     OnDevice on("vox_hip_linear_i8", device);
     if (!on.ok) return -1;
     const int ldq = i8_ldq(K);
     int8_t *xq = (int8_t *)ws;
-    const bool wide = K % 16 == 0 && w_stride % 16 == 0 && aligned(w, 16);
+    const bool wide = i8_wide(K, w, w_stride);
     const I8Plan p = i8_plan(rows, K, N, wide);
     float *xs = (float *)((char *)ws + p.scale_at);
     LinearI8Args a{xq, xs, w, w_stride, w_scale, bias, y, y_stride, (int)rows, K, N, ldq, (int *)((char *)ws + p.part_at), p.splits};

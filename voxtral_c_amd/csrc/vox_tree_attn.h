@@ -243,18 +243,16 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, (DP == 256 || (ATTN_SPLIT<T, SHARE
     const int group = chunk * 8 + (in & 7), rb = in >> 3;
     const int b = blockIdx.y, split = group / a.Hk, kvh = group - split * a.Hk;
     if (split >= plan.splits) return;
-    const TileRange tr = tile_range<KT>(a, b, plan.splits, KW);
-    const int t_begin = split * tr.per, t_end = min(t_begin + tr.per, tr.n_all);
-    if (t_begin >= t_end) return;
     const int R = a.T * a.G, row0 = rb * ROWS;
     const int kw = SHARED ? 0 : wave, rw = SHARED ? (wave + split) & (ATTN_WAVES - 1) : 0;       // (idle waves on another SIMD from split to split)
     const int wrow0 = row0 + rw * WROWS;
     const bool idle = wrow0 >= R;                            // (the last workgroup's waves behind the last row)
 
-    // this lane's query rows; a negative scale goes into Q's sign
+    // this lane's query rows, requested in front of the cache's length; a negative scale goes into Q's sign
     constexpr bool QLDS = !SHARED && (sizeof(T) == 4 || DP == 256);
     mvec qf[QLDS ? 1 : RT][QLDS ? 1 : MS][SPLIT ? 3 : 1];
     kvec *qs = reinterpret_cast<kvec *>(lds);                // [RT][KS][64 lanes]
+    kvec qr[RT][KS];
     int row_depth[RT], row_node[RT];
 #pragma unroll
     for (int t = 0; t < RT; t++) {
@@ -262,21 +260,30 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, (DP == 256 || (ATTN_SPLIT<T, SHARE
         row_node[t] = node;
         row_depth[t] = row < R ? min(a.depth[(size_t)b * a.T + node], 1 << 30) : -1;
         const T *q = (const T *)a.q + b * a.q_sb + node * a.q_st + h * a.q_sh;
-        auto load = [&](int d) {
-            kvec x = kvec(T(0.f));
-            if (row < R && d < a.D) x = *reinterpret_cast<const kvec *>(q + d);
-            return a.scale < 0.f ? -x : x;
-        };
 #pragma unroll
-        for (int s = 0; s < MS; s++) {
-            const int d = s * 4 * MU + c * MU;
-            if constexpr (SPLIT) {
-                const kvec x[2] = {load(d), load(d + 4)};
-                split3<mvec>([&](int i) { return x[i >> 2][i & 3]; }, qf[t][s][0], qf[t][s][1], qf[t][s][2]);
-            } else if constexpr (!QLDS) qf[t][s][0] = load(d);
-            else if (kw == 0) qs[(t * KS + s) * 64 + lane] = load(d);
+        for (int i = 0; i < KS; i++) {
+            // (a matrix operand takes MU values in a row: two of f32's loads, where it is split)
+            const int d = SPLIT ? (i >> 1) * 4 * MU + c * MU + (i & 1) * U : i * 4 * U + c * U;
+            qr[t][i] = kvec(T(0.f));
+            if (row < R && d < a.D && (!QLDS || kw == 0)) qr[t][i] = *reinterpret_cast<const kvec *>(q + d);
         }
     }
+    const TileRange tr = tile_range<KT>(a, b, plan.splits, KW);
+    const int t_begin = split * tr.per, t_end = min(t_begin + tr.per, tr.n_all);
+    if (t_begin >= t_end) return;
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int i = 0; i < KS; i++)
+            if (a.scale < 0.f) qr[t][i] = -qr[t][i];
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int s = 0; s < MS; s++) {
+            if constexpr (SPLIT) split3<mvec>([&](int i) { return qr[t][s * 2 + (i >> 2)][i & 3]; }, qf[t][s][0], qf[t][s][1], qf[t][s][2]);
+            else if constexpr (!QLDS) qf[t][s][0] = qr[t][s];
+            else if (kw == 0) qs[(t * KS + s) * 64 + lane] = qr[t][s];
+        }
     const float scale2 = fabsf(a.scale) * LOG2E;
 
     const char *kc = (const char *)((const T *)a.kc + b * a.kc_sb + kvh * a.kc_sh), *vc = (const char *)((const T *)a.vc + b * a.vc_sb + kvh * a.vc_sh);
@@ -290,20 +297,8 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, (DP == 256 || (ATTN_SPLIT<T, SHARE
     // end.  A tile of
     // those that the ring does not break is plain: its rows follow each other, and a lane's offsets within it are the same for every tile.
     const int edge = (int)max(tr.len + 1 - a.window - tr.first, (int64_t)-(1 << 30));            // first position of a window at depth 0, from `first`
-    int deepest = 0;
-    if (a.window > 0) {                                      // (of this workgroup's rows: the deepest node's window begins last)
-        __shared__ int depths[RW];
-#pragma unroll
-        for (int r = 0; r < RT; r++) deepest = max(deepest, row_depth[r]);
-#pragma unroll
-        for (int i = 1; i < 16; i <<= 1) deepest = max(deepest, __shfl_xor(deepest, i, 64));
-        if (lane == 0) depths[rw] = deepest;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < RW; i++) deepest = max(deepest, depths[i]);
-        deepest = __builtin_amdgcn_readfirstlane(deepest);
-    }
-    const int full_begin = a.window > 0 && edge + deepest > 0 ? (edge + deepest - 1) / KT + 1 : 0, full_end = tr.cached / KT;
+    const int full_end = tr.cached / KT;
+    int deepest = 0, full_begin = 0;                         // (behind the first tiles' loads)
     auto is_masked = [&](int t) { return t < full_begin || t >= full_end; };
     auto is_plain = [&](int t) { return a.D == DP && t < full_end && slot_of(t) + KT <= (unsigned)a.cap; };
     auto tile_at = [&](int t) {
@@ -334,9 +329,12 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, (DP == 256 || (ATTN_SPLIT<T, SHARE
         if (t >= tr.n_cache) {
             const int off = (t - tr.n_cache) * KT;
             bits = (unsigned)(a.ancestors[((size_t)b * a.T + row_node[r]) * a.W + (off >> 6)] >> (off & 63));
-            if (a.window > 0)
-                for (int j = 0; j < count; j++)
-                    if (a.depth[(size_t)b * a.T + off + j] <= row_depth[r] - a.window) bits &= ~(1u << j);
+            if (a.window > 0) {
+                const int d = (lane & 31) < count ? a.depth[(size_t)b * a.T + off + (lane & 31)] : 0x7fffffff;
+                if (__any(d <= deepest - a.window))          // (only trees that are deeper than the window)
+                    for (int j = 0; j < count; j++)
+                        if (__builtin_amdgcn_readlane(d, j) <= row_depth[r] - a.window) bits &= ~(1u << j);
+            }
         } else if (a.window > 0) {
             const int below = edge + row_depth[r] - t * KT;  // keys in front of the row's window
             bits = below >= 32 ? 0u : below <= 0 ? 0xffffffffu : 0xffffffffu << below;
@@ -459,6 +457,21 @@ __global__ __launch_bounds__(64 * ATTN_WAVES, (DP == 256 || (ATTN_SPLIT<T, SHARE
     } else {
         if (QLDS) __syncthreads();
         if (t < t_end) { load_k(t); load_v(t); }
+    }
+    if (a.window > 0) {                                      // (of this workgroup's rows: the deepest node's window begins last)
+#pragma unroll
+        for (int r = 0; r < RT; r++) deepest = max(deepest, row_depth[r]);
+#pragma unroll
+        for (int i = 1; i < 16; i <<= 1) deepest = max(deepest, __shfl_xor(deepest, i, 64));
+        if constexpr (RW > 1) {
+            __shared__ int depths[RW];
+            if (lane == 0) depths[rw] = deepest;
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");    // (the first tiles stay on their way)
+#pragma unroll
+            for (int i = 0; i < RW; i++) deepest = max(deepest, depths[i]);
+        }
+        deepest = __builtin_amdgcn_readfirstlane(deepest);
+        full_begin = edge + deepest > 0 ? (edge + deepest - 1) / KT + 1 : 0;
     }
     for (; t < t_end; t += KW) {
         const bool more = t + KW < t_end, masked = is_masked(t);

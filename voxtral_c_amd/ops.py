@@ -40,7 +40,7 @@ hip.vox_hip_token_scores_workspace.argtypes = [_i, _q, _i, _i]
 hip.vox_hip_token_scores_workspace.restype = _q
 hip.vox_hip_token_scores.argtypes = [_i, _p, _q, _q, _i, _p, _i, _i] + [_p] * 6 + [C.c_size_t, _i, _p]
 hip.vox_hip_quantize_rows_i8.argtypes = [_i, _p, _q, _q, _i, _p, _p, _i, _p]
-hip.vox_hip_linear_i8_workspace.argtypes = [_i, _q, _i, _i]
+hip.vox_hip_linear_i8_workspace.argtypes = [_i, _q, _i, _i, _p, _q]
 hip.vox_hip_linear_i8_workspace.restype = _q
 hip.vox_hip_linear_i8.argtypes = [_i, _p, _q, _q, _i, _i, _p, _q, _p, _p, _p, _q, _p, C.c_size_t, _i, _p]
 _Strides = _q * 4
@@ -159,7 +159,8 @@ def tree_accept(tokens, choices, root_choice, parents, ancestors, depth, cache_l
     root_choice, cache_len = _table(who, "root_choice", root_choice, (B,)), _table(who, "cache_len", cache_len, (B,))
     ancestors = _table(who, "ancestors", ancestors, (B, T, (T + 63) // 64), torch.int64)
     d = _device(who, tokens, choices, root_choice, parents, ancestors, depth, cache_len)
-    path, n, after, new_len = torch.empty_like(tokens), torch.empty_like(root_choice), torch.empty_like(root_choice), torch.empty_like(root_choice)
+    path = torch.empty_like(tokens)
+    n, after, new_len = root_choice.new_empty((3, B)).unbind()
     if hip.vox_hip_tree_accept(tokens.data_ptr(), choices.data_ptr(), root_choice.data_ptr(), parents.data_ptr(), ancestors.data_ptr(), depth.data_ptr(),
                                cache_len.data_ptr(), B, T, path.data_ptr(), n.data_ptr(), after.data_ptr(), new_len.data_ptr(), d, _stream(d)):
         _error(who)
@@ -252,9 +253,10 @@ def linear_i8(x, w, w_scale, bias=None):
         raise ValueError(f"{who}: w_scale needs gradients: there is no backward pass (use torch.no_grad())")
     d = _device(who, x, w, w_scale, *(() if bias is None else (bias,)))
     y = x.new_empty((M, N))
-    need = hip.vox_hip_linear_i8_workspace(number, M, K, N)
-    ws = x.new_empty(max(need, 1), dtype=torch.uint8)
-    if need < 0 or hip.vox_hip_linear_i8(number, x.data_ptr(), x.stride(0), M, K, N, w.data_ptr(), w.stride(0), w_scale.data_ptr(),
-                                         None if bias is None else bias.data_ptr(), y.data_ptr(), N, ws.data_ptr(), need, d, _stream(d)):
+    wp, wst = w.data_ptr(), w.stride(0)
+    need = hip.vox_hip_linear_i8_workspace(number, M, K, N, wp, wst)
+    ws = x.new_empty(need, dtype=torch.uint8) if need > 0 else None
+    if need < 0 or hip.vox_hip_linear_i8(number, x.data_ptr(), x.stride(0), M, K, N, wp, wst, w_scale.data_ptr(),
+                                         None if bias is None else bias.data_ptr(), y.data_ptr(), N, None if ws is None else ws.data_ptr(), need, d, _stream(d)):
         _error(who)
     return y
