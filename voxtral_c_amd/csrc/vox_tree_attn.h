@@ -96,10 +96,13 @@ template <typename T> __global__ __launch_bounds__(256) void k_tree_attn_scalar(
 //                                A operand in the same order: lane m of a 16-lane row takes VU consecutive dimensions (16 m VU ..) of the keys
 //                                4 c + r and supplies one of them to each of E products.
 // Two ways to the keys:
-//   own      (up to 32 rows) every wave has keys of its own, straight from memory into the registers that the matrix instruction reads, 16 bytes per
-//            lane; K of the next step is requested when the scores are done, V when the outputs are.  Bound by the read of the cache.
+//   own      (up to 16 rows, 32 where a head has up to 64 dimensions) every wave has keys of its own, straight from memory into the registers that the
+//            matrix instruction reads, 16 bytes per lane; K of the next step is requested when the scores are done, V when the outputs are.  Bound by
+//            the read of the cache, and for short caches by latency: 2 nodes x 4 heads over 232 keys, f32: 11.2 us, the join of 4 parts 3.9 us.
 //   shared   (more rows) the four waves have rows of their own and share the steps' keys in LDS, which global_load_lds fills STAGES steps ahead:
-//            nothing of it is in registers, and the cache is read once per 64 or 128 rows.  Bound by the read, or by the products of f32.
+//            nothing of it is in registers, and the cache is read once per 64 or 128 rows.  24 nodes x 4 heads over 4 x 40000 keys, bf16: 127 us for 557 MB
+//            (4.4 TB/s), bound by the read; 64 nodes x 4 heads over 2 x 8191 keys, f32: 175 us, bound by the vector unit, which splits the numbers (below).
+// Where both would do, 32 rows of 128 dimensions over 4 x 16000 keys: own 78 us, shared 57 in bf16, 152 and 125 in f32.
 // Each wave runs its own online softmax (one maximum and sum per row); waves with different keys are joined through LDS at the end, the parts of a
 // long cache by k_tree_attn_join.
 template <typename T> struct AttnType;
@@ -129,7 +132,8 @@ template <> struct AttnType<f16_t> {
 constexpr int ATTN_WAVES = 4;
 // Shared keys of f32 are multiplied on the bf16 pipe: a number is exactly the sum of three bf16 ones (8 of its 24 bits each), and of the nine
 // products the six down to 2^-16 of the largest are taken, the rest is below 2^-24.  An f32 matrix instruction takes the vector unit's cycles (measured:
-// the two run one after the other, 0.23 + 0.23 ms -> 0.46 ms), a bf16 one does not, and six of them take 6 x 17 cycles where f32 takes 8 x 33.
+// the two run one after the other, 0.23 + 0.23 ms -> 0.46 ms), a bf16 one does not, and six of them take 6 x 17 cycles where f32 takes 8 x 33:
+// 64 rows over 4 x 16000 keys 163 -> 142 us, 32 rows 152 -> 125.  Splitting each key once per workgroup into LDS instead of in every wave was slower (178 us).
 template <typename T, bool SHARED> constexpr bool ATTN_SPLIT = SHARED && sizeof(T) == 4;
 template <typename T, bool SHARED> constexpr int ATTN_KT = SHARED || sizeof(T) == 2 ? 32 : 16;              // keys of a step
 template <typename T> constexpr int ATTN_STAGES = sizeof(T) == 4 ? 2 : 3;                                   // (two workgroups per CU)
