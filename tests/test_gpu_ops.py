@@ -705,3 +705,53 @@ def test_attention_over_the_engines_own_ring():
         v.hip.vox_hip_sync(e)
         w = ref.attention(c["q"], c["k"], c["v"], torch.as_tensor(host[0]), torch.as_tensor(host[1]), [n], c["ancestors"].cpu().numpy(), c["depth"].cpu().numpy(), D ** -0.5, dims.dec_window)
         assert (np.abs(out.cpu().double().numpy() - w[0]) <= ref.attention_bound(w[0], w[2], w[4], F32)).all() and (np.abs(lse.cpu().double().numpy() - w[1]) <= w[3]).all()
+
+
+class HandsBack:
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+def test_compiled_calls_and_their_python_twins_agree(monkeypatch):
+    """What the compiled calls take and what they hand back run the same kernels: equal bits, and ordinary arguments are taken."""
+    for dtype in (F32, BF16, F16):
+        c = captured_state(41, dtype)
+        want = verification_pass(c)
+        assert ops._call.quantize_rows_i8(randn(np.random.default_rng(1), 3, 40, dtype=dtype)) is not None
+        with monkeypatch.context() as m:
+            m.setattr(ops, "_call", HandsBack())
+            assert same(want, verification_pass(c))
+
+
+def test_wrong_calls_on_the_gpu_are_refused():
+    rng = np.random.default_rng(3)
+    q, k, kc = randn(rng, 2, 3, 4, 16), randn(rng, 2, 3, 2, 16), randn(rng, 2, 9, 2, 16)
+    length = dev(np.array([4, 20], np.int32))
+    words, depth = ops.tree_plan(dev(np.array([[-1, 0, 1], [-1, -1, 0]], np.int32)))
+    good = [q, k, k.clone(), kc, kc.clone(), length, words, depth]
+    out = ops.tree_attention(*good)
+    assert torch.equal(out, ops.tree_attention(*good, scale=16 ** -0.5, window=0)) and torch.equal(out, ops.tree_attention(*good, window=2 ** 40))
+    for i, bad in ((0, q.half()), (0, q[:, :, :3]), (0, q.cpu()), (1, k[:1]), (2, k.double()), (3, kc[..., :8]), (4, kc.transpose(2, 3)), (5, length.long()), (5, length[:1]),
+                   (6, words.int()), (7, depth[:, :2]), (7, depth.cpu()), (1, k.clone().requires_grad_())):
+        with pytest.raises(ValueError, match="tree_attention"):
+            ops.tree_attention(*good[:i], bad, *good[i + 1:])
+    for scale in (0.0, math.inf, math.nan):
+        with pytest.raises(v.VoxError, match="scale"):
+            ops.tree_attention(*good, scale=scale)
+    spread = torch.stack([depth, depth], 2)[:, :, 0]                   # a table that is not contiguous is copied
+    assert torch.equal(out, ops.tree_attention(*good[:7], spread))
+    x, w, s = randn(rng, 3, 32), torch.ones(5, 32, dtype=torch.int8, device="cuda"), torch.ones(5, device="cuda")
+    assert ops.linear_i8(x, w, s).shape == (3, 5)
+    for args in ((x, w[:, :16], s), (x, w, s[:4]), (x, w.float(), s), (x, w, s, s[:2]), (x, w, s, s.half()), (x, w, s.cpu()), (x, w, s.clone().requires_grad_()), (x.double(), w, s)):
+        with pytest.raises(ValueError, match="linear_i8"):
+            ops.linear_i8(*args)
+    for args in ((x, None, 33), (x, None, -1), (x, dev(np.zeros((2, 1), np.int32))), (x, dev(np.zeros((3, 1), np.int64))), (x[0],), (x.t(),)):
+        with pytest.raises(ValueError, match="token_scores"):
+            ops.token_scores(*args)
+    t = dev(np.zeros((2, 3), np.int32))
+    with pytest.raises(ValueError, match="tree_accept"):
+        ops.tree_accept(t, t, length, t, words, depth[:1], length)
+    n = dev(np.ones(2, np.int32))
+    for a in ((k, k, kc[:, :2], kc[:, :2]), (k, k, kc[:, :1].expand(2, 9, 2, 16), kc), (k, k, kc.half(), kc), (k, k.cpu(), kc, kc)):
+        with pytest.raises(ValueError, match="tree_commit"):
+            ops.tree_commit(*a, t, n, length)

@@ -21,7 +21,7 @@ from collections import namedtuple
 
 import torch
 
-from . import VoxError, hip
+from . import VoxError, _ops_call as _call, hip
 
 MAX_NODES = 256
 MAX_TOP = 64
@@ -92,6 +92,12 @@ def _stream(device):
     return _raw_stream(device) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
 
 
+# The compiled calls (csrc/vox_ops_call.cpp) take what is in order; what they hand back as None is done or refused here.
+_call.bind(_raw_stream or _stream, *(C.cast(getattr(hip, "vox_hip_" + n), _p).value for n in (
+    "tree_plan", "tree_attention_workspace", "tree_attention", "tree_accept", "tree_commit", "token_scores_workspace", "token_scores",
+    "quantize_rows_i8", "linear_i8_workspace", "linear_i8")))
+
+
 def _nodes(who, shape):
     if len(shape) < 2 or shape[1] > MAX_NODES:
         raise ValueError(f"{who}: shape {tuple(shape)}: [batch, nodes, ..] with at most {MAX_NODES} nodes is needed")
@@ -100,6 +106,9 @@ def _nodes(who, shape):
 def tree_plan(parents, n_nodes=None):
     """Ancestor sets int64 [batch, nodes, ceil(nodes / 64)] and depths int32 [batch, nodes] of draft trees: parents int32 [batch, nodes], -1 for
     the cache's end, otherwise an earlier node; n_nodes int32 [batch] where trees are shorter than the padded width."""
+    done = _call.tree_plan(parents, n_nodes)
+    if done is not None:
+        return done
     who = "tree_plan"
     _nodes(who, parents.shape)
     B, T = parents.shape if parents.dim() == 2 else (-1, -1)
@@ -119,6 +128,9 @@ def tree_attention(q, k, v, k_cache, v_cache, cache_len, ancestors, depth, scale
     caches [batch, cap, kv_heads, dim] (position p in row p % cap), cache_len int32 [batch], the tables of tree_plan (or any other mask of
     that form).  window <= 0: none, otherwise a node sees positions above its own - window.  Rows that see nothing are zeros.
     Returns out like q, with return_lse (out, float32 [batch, nodes, heads])."""
+    done = _call.tree_attention(q, k, v, k_cache, v_cache, cache_len, ancestors, depth, scale, window, return_lse)
+    if done is not None:
+        return done
     who = "tree_attention"
     if q.dim() != 4 or k_cache.dim() != 4 or k.dim() != 4:
         raise ValueError(f"{who}: q, k and the caches have 4 dimensions: got {q.dim()}, {k.dim()}, {k_cache.dim()}")
@@ -149,6 +161,9 @@ def tree_accept(tokens, choices, root_choice, parents, ancestors, depth, cache_l
     """The drafted path that the model agrees with: tokens and choices (the model's token behind each node) int32 [batch, nodes], root_choice
     (its token behind the cache) int32 [batch].  Returns path int32 [batch, nodes] (-1 behind the accepted nodes), their number,
     the model's token behind the path, and the cache's new length, int32 [batch] each."""
+    done = _call.tree_accept(tokens, choices, root_choice, parents, ancestors, depth, cache_len)
+    if done is not None:
+        return done
     who = "tree_accept"
     _nodes(who, tokens.shape)
     B, T = tokens.shape if tokens.dim() == 2 else (-1, -1)
@@ -173,6 +188,8 @@ def tree_commit(k, v, k_cache, v_cache, path, n_accepted, cache_len):
     who = "tree_commit"
     if k.dim() == 4:
         k, v, k_cache, v_cache = k[None], v[None], k_cache[None], v_cache[None]
+    if _call.tree_commit(k, v, k_cache, v_cache, path, n_accepted, cache_len):
+        return
     if k.dim() != 5 or k_cache.dim() != 5:
         raise ValueError(f"{who}: k {tuple(k.shape)}, k_cache {tuple(k_cache.shape)}: [layers,] batch, rows, kv_heads, dim are needed")
     L, B, T, Hk, D = k.shape
@@ -199,6 +216,9 @@ def token_scores(logits, tokens=None, top=0):
     """Scores of rows of logits [rows, vocab]: log probabilities of `tokens` int32 [rows, given] (or [rows]), the distribution's entropy and
     log-sum [rows], and the `top` largest logits' indexes and log probabilities [rows, top], equal ones by the lowest index.  An id outside
     the vocabulary scores -inf."""
+    done = _call.token_scores(logits, tokens, top)
+    if done is not None:
+        return TokenScores(*done)
     who = "token_scores"
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"{who}: logits have the shape {tuple(logits.shape)}: [rows, vocab] is needed")
@@ -226,6 +246,9 @@ def token_scores(logits, tokens=None, top=0):
 def quantize_rows_i8(x):
     """x [rows, K] -> (int8 [rows, K], float32 scales [rows]): scale = largest magnitude / 127, whole numbers to nearest, ties to even.  With a
     weight matrix [outputs, inputs] this gives linear_i8's w and w_scale."""
+    done = _call.quantize_rows_i8(x)
+    if done is not None:
+        return done
     who = "quantize_rows_i8"
     if x.dim() != 2 or not 1 <= x.shape[1] <= 131072:
         raise ValueError(f"{who}: x has the shape {tuple(x.shape)}: [rows, K] with K of 1 to 131072 is needed")
@@ -240,6 +263,9 @@ def quantize_rows_i8(x):
 def linear_i8(x, w, w_scale, bias=None):
     """y [rows, outputs] in x's type = x [rows, inputs], quantised row by row as quantize_rows_i8 does, times w int8 [outputs, inputs] with one float32
     scale per output, plus bias [outputs] in x's type.  The sum of the whole numbers is exact."""
+    done = _call.linear_i8(x, w, w_scale, bias)
+    if done is not None:
+        return done
     who = "linear_i8"
     if x.dim() != 2 or not 1 <= x.shape[1] <= 131072 or w.dim() != 2:
         raise ValueError(f"{who}: x has the shape {tuple(x.shape)}, w {tuple(w.shape)}: [rows, K] and [outputs, K] with K of 1 to 131072 are needed")
