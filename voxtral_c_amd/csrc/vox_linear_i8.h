@@ -117,7 +117,7 @@ template <typename T> __global__ __launch_bounds__(256) void k_linear_i8_bytes(L
 // A workgroup makes 16 output channels of MT x 16 rows; its waves split K and their whole-number sums are added through LDS (exact in any order).
 // v_mfma_i32_16x16x64_i8 with the weights as A operand: lane = (channel lane % 16, 16 bytes of K), loaded straight from the row-major matrix, 64 bytes of
 // each of 16 rows per instruction and two neighbouring instructions per 128-byte line.  25 x 5120 x 1280: 8.5 us, 0.8 TB/s of weights (80 workgroups; operands
-// four steps ahead changed nothing), 14 us a call with the quantiser's launch.
+// four steps ahead changed nothing), 11.4 us a call with the quantiser's launch.
 constexpr int I8_ROWS_WAVES = 8;
 template <typename T, int MT> __global__ __launch_bounds__(64 * I8_ROWS_WAVES) void k_linear_i8_rows(LinearI8Args a) {
     __shared__ i32x4 part[I8_ROWS_WAVES][MT][64];
@@ -156,7 +156,7 @@ template <typename T, int MT> __global__ __launch_bounds__(64 * I8_ROWS_WAVES) v
 
 // The same in one launch for a few rows (single tokens): every workgroup quantises all of x into its LDS while its first weights are on their way.  Up
 // to I8_FEW elements of x: 32 per thread, about a microsecond; a launch of its own costs 3 us (1 x 1280 x 6144,
-// f32: 13.9 -> 9.7 us a call; the kernel 6.6 us, 1.2 TB/s of weights).
+// f32: 13.9 -> 10.9 us a call then, 5.8 now; 1.4 TB/s of weights).
 constexpr int I8_FEW = 16384, I8_FEW_ROWS = 16, I8_FEW_AHEAD = 2;
 template <typename T, int N> __global__ __launch_bounds__(64 * I8_ROWS_WAVES) void k_linear_i8_few(LinearI8Args a, const T *x, int64_t x_stride) {
     __shared__ i32x4 part[I8_ROWS_WAVES][64];

@@ -4,7 +4,7 @@
 // elements of its share as a sorted list with one entry per lane, and both are joined over lanes, waves and (few long rows) parts of a row.
 // Measured, vocabulary 131072, logits read once in a call: 386 rows of f32, top 4: 49 us (4.1 TB/s; the kernel 43 us, 4.7 TB/s, joining the parts
 // 6 us); 1501 rows of bf16, top 32: 100 us (3.9 TB/s: a bf16 logit costs the same vector work as an f32 one at half the bytes, and here both count).
-// One row, top 8: 7.7 + 5.1 us for parts and join, bound by latency, 18.6 us a call from Python, bound by the host.
+// One row, top 8: 7.7 + 5.1 us for parts and join, bound by latency; 12 us a call from Python.
 #pragma once
 #include "vox_ops_common.h"
 
