@@ -148,3 +148,15 @@ def test_c_entries_refuse_before_any_launch():
     assert v.hip.vox_hip_token_scores_workspace(0, far, 1, 0) == -1 and "rows" in err()
     if v.device_count() == 0:
         assert v.hip.vox_hip_tree_plan(fake, None, 1, 4, fake, fake, 0, None) == -1 and "no such device" in err()
+
+
+def test_compiled_calls_hand_back_what_they_do_not_take():
+    """Tensors on the CPU, other things than tensors, wrong counts: None, so that the Python call says what is wrong."""
+    c, x, t = ops._call, zeros(2, 16), zeros(2, 3, dtype=torch.int32)
+    q = zeros(1, 2, 4, 16)
+    for done in (c.tree_plan(t, None), c.tree_plan([1], None), c.tree_plan(t), c.tree_plan(t, 3), c.quantize_rows_i8(x), c.quantize_rows_i8(None), c.quantize_rows_i8(),
+                 c.linear_i8(x, x, x, None), c.linear_i8(x, x.char(), x[0], 1.0), c.token_scores(x, None, 0), c.token_scores(x, None, 2 ** 80), c.token_scores(x, None, 1.5),
+                 c.tree_accept(*[t] * 7), c.tree_commit(*[q[None]] * 4, t, t, t), c.tree_attention(*[q] * 8, None, 0, True), c.tree_attention(*[q] * 8, "1", None, 1)):
+        assert done is None
+    with pytest.raises(TypeError, match="arguments"):
+        c.bind(print, 1)

@@ -15,7 +15,9 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
+#include <cstring>
 
 #include "../../include/vox_hip_ops.h"
 
