@@ -1,0 +1,89 @@
+"""GPU: calls of the draft-verification operators at the edges of what their definitions allow, against 64 bits (test_gpu_ops.py has the ordinary ones)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import voxtral_c_amd as v
+from voxtral_c_amd import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F32, BF16, F16, I32 = torch.float32, torch.bfloat16, torch.float16, torch.int32
+
+
+@pytest.fixture(autouse=True)
+def need_gpu():
+    if v.device_count() < 1:
+        pytest.fail("no HIP device: the product has no CPU fallback")
+
+
+# ---- scores: tokens switched off with the type's lowest number -----------------------------------------------------------------
+def check_switched_off(x, live, tokens, top):
+    """x [rows, V], live [V] truth values: the tokens that are not switched off.  The tolerances are those of ordinary rows, from the live tokens' span."""
+    g = ops.token_scores(x, tokens, top)
+    assert not any(torch.isnan(t).any() for t in (g.logprob, g.entropy, g.lse, g.top_logprob))
+    x64 = x.cpu().double().numpy()
+    m = x64.max(1, keepdims=True)
+    log1 = np.log(np.exp(x64 - m).sum(1, keepdims=True))               # (apart from m, next to which it may be nothing)
+    lse, lp = (m + log1)[:, 0], (x64 - m) - log1
+    p = np.exp(lp)
+    entropy = -np.where(p > 0, p * lp, 0).sum(1)
+    index = np.argsort(-x64, axis=1, kind="stable")[:, :top]
+    V, e = x.shape[1], 2.0 ** -24
+    size = log1 + (np.ptp(x64[:, live]) if live.any() else 0.0)
+    # Exponents are off by 2 e of their size (17 at most, smaller terms do not matter), sums by their depth; the maximum's addition, x - max and log1p
+    # by 3 e of their sizes.
+    sum_off = (2 * 17 + 4 + V / 64 + 64) * e
+
+    def near(got, want, tol):
+        off = np.abs(got.cpu().double().numpy() - want)
+        assert (off <= tol).all(), (off - tol).max()
+    near(g.lse, lse, sum_off + 3 * e * np.abs(lse))
+    near(g.entropy, entropy, sum_off * (2 + entropy) * 2 + 3 * e * size[:, 0])
+    given, best = np.take_along_axis(lp, tokens.cpu().numpy(), 1), np.take_along_axis(lp, index, 1)
+    near(g.logprob, given, sum_off + 3 * e * (size + np.abs(given)))
+    near(g.top_logprob, best, sum_off + 3 * e * (size + np.abs(best)))
+    assert np.array_equal(g.top_index.cpu().numpy(), index)
+    return g
+
+
+def live_tokens(V, kind, rng):
+    """Which tokens stay: behind the first loads of a row, but for one wave's share, the last few, the first few, every 97th, none."""
+    at = np.arange(V)
+    return {"behind": at >= min(V - 3, 9000), "wave": (at // 64) % 4 != 1, "wave4": (at // 256) % 4 != 1, "wave8": (at // 512) % 4 != 2, "last": at >= V - 5, "first": at < 5,
+            "some": at % 97 == 3, "none": at < 0}[kind]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("kind", ["behind", "wave", "wave4", "wave8", "last", "first", "some", "none"])
+@pytest.mark.parametrize("R,V", [(3, 131072), (1, 131072), (700, 2048), (2, 40003), (701, 4099), (1, 70)])
+def test_token_scores_tokens_switched_off_with_the_lowest_number(R, V, kind, dtype):
+    """finfo.min in place of -inf: an ordinary row over the tokens that stay, whoever of lanes, waves and parts holds nothing else."""
+    rng = np.random.default_rng(V + R)
+    live = live_tokens(V, kind, rng)
+    x = torch.full((R, V), torch.finfo(dtype).min, dtype=dtype, device=DEV)
+    x[:, torch.as_tensor(live, device=DEV)] = torch.as_tensor(rng.standard_normal((R, int(live.sum()))).astype(np.float32) * 3).to(dtype).to(DEV)
+    tokens = torch.as_tensor(rng.integers(0, V, (R, 2)).astype(np.int32)).to(DEV)
+    check_switched_off(x, live, tokens, min(5, V))
+
+
+@pytest.mark.parametrize("V", [16384, 131072, 40003])
+def test_token_scores_rising_steps_of_large_numbers(V):
+    """Rows that climb from the lowest number over large steps to an ordinary end, and past it to the largest number: every step leaves the former sums nothing."""
+    x = torch.empty(2, V, device=DEV)
+    steps = -torch.logspace(38.5, 3, V, dtype=torch.float64)
+    x[0] = steps.clamp(min=torch.finfo(F32).min).float().to(DEV)
+    x[0, -100:] = torch.linspace(0, 5, 100, device=DEV)
+    x[1] = x[0]
+    x[1, V // 2] = torch.finfo(F32).max                                # one token has all the probability
+    g = ops.token_scores(x, torch.tensor([[V - 1], [V // 2]], dtype=I32, device=DEV), 2)
+    z = np.linspace(0, 5, 100).astype(np.float32).astype(np.float64)
+    lse = np.log(np.exp(z).sum())
+    entropy = lse - (np.exp(z - lse) * z).sum()
+    e = 2.0 ** -24
+    tol = (2 * 17 + 4 + V / 64 + 64) * e
+    assert abs(float(g.lse[0]) - lse) <= tol + 3 * e * 15 and abs(float(g.entropy[0]) - entropy) <= tol * (2 + entropy) * 2 + 3 * e * 15
+    assert abs(float(g.logprob[0, 0]) - (5 - lse)) <= tol + 3 * e * 15 and g.top_index[:, 0].tolist() == [V - 1, V // 2]
+    assert float(g.lse[1]) == torch.finfo(F32).max and float(g.entropy[1]) == 0 and float(g.logprob[1, 0]) == 0

@@ -18,13 +18,16 @@ namespace vox {
 struct RowSum {
     float m, s, t;
 };
+// A distance below -200 counts as -200: its weight e^d is 0 in any case, and 0 times a distance as large as the type's lowest number, or times a sum
+// of such, would be NaN.
+constexpr float SC_FAR = -200.f;
 __device__ __forceinline__ float exp_fast(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896340736f); }
 __device__ __forceinline__ RowSum row_join(const RowSum a, const RowSum b) {
     if (a.m != a.m || b.m != b.m) return {NAN, NAN, NAN};
     const bool first = a.m >= b.m;
     const RowSum hi = first ? a : b, lo = first ? b : a;
     if (lo.m == -INFINITY || hi.m == INFINITY) return hi;
-    const float d = lo.m - hi.m, f = expf(d), l = 1.f + lo.s;
+    const float d = fmaxf(lo.m - hi.m, SC_FAR), f = expf(d), l = 1.f + lo.s;
     return {hi.m, hi.s + f * l, hi.t + f * (lo.t + d * l)};
 }
 
@@ -225,7 +228,7 @@ template <typename T, int N> __global__ __launch_bounds__(SC_THREADS) void k_tok
         const float peak = wave_max_dpp(most);
         if (peak > m) {
             if (m != -INFINITY) {                            // the old maximum's own term joins the others
-                const float d = m - peak, e = exp_fast(d);
+                const float d = fmaxf(m - peak, SC_FAR), e = exp_fast(d);
                 s += lane == 0 ? 1.f : 0.f;
                 t = e * (t + d * s);
                 s *= e;
@@ -240,7 +243,7 @@ template <typename T, int N> __global__ __launch_bounds__(SC_THREADS) void k_tok
                     const float d = f[u][j] - m, e = skip ? 0.f : exp_fast(d);
                     own = own && !skip;
                     s += e;
-                    t += e * fmaxf(d, -200.f);               // (e^-inf * -inf is 0 here)
+                    t += e * fmaxf(d, SC_FAR);               // (e^-inf * -inf is 0 here)
                 }
         } else {
             const float base = m == -INFINITY ? 0.f : m;
@@ -250,7 +253,7 @@ template <typename T, int N> __global__ __launch_bounds__(SC_THREADS) void k_tok
                 for (int j = 0; j < N; j++) {
                     const float d = f[u][j] - base, e = exp_fast(d);
                     s += e;
-                    t += e * fmaxf(d, -200.f);
+                    t += e * fmaxf(d, SC_FAR);
                 }
         }
         if (a.top > 0) {
