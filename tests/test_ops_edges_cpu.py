@@ -1,0 +1,43 @@
+"""CPU: what the draft-verification operators refuse at the edges of their arguments, and how they are built and loaded."""
+import pytest
+import torch
+
+from voxtral_c_amd import ops
+
+I32 = torch.int32
+
+
+def meta(*shape, dtype=torch.float32):
+    return torch.empty(shape, dtype=dtype, device="meta")              # (shapes and types without memory)
+
+
+FAR = 2 ** 32 + 3                                                      # a size whose low 32 bits are an ordinary one
+
+
+def attention_of(B, T, H, D, Hk, cap):
+    m = meta
+    return (m(B, T, H, D), m(B, T, Hk, D), m(B, T, Hk, D), m(B, cap, Hk, D), m(B, cap, Hk, D), m(B, dtype=I32), m(B, T, (T + 63) // 64, dtype=torch.int64), m(B, T, dtype=I32))
+
+
+def commit_of(L, B, T, Hk, D, cap):
+    k, c = meta(L, B, T, Hk, D), meta(L, B, cap, Hk, D)
+    return k, k, c, c, meta(B, T, dtype=I32), meta(B, dtype=I32), meta(B, dtype=I32)
+
+
+def accept_of(B, T):
+    t, r = meta(B, T, dtype=I32), meta(B, dtype=I32)
+    return t, t, r, t, meta(B, T, 1, dtype=torch.int64), t, r
+
+
+@pytest.mark.parametrize("call,args", [
+    ("tree_plan", (meta(FAR, 1, dtype=I32),)), ("tree_plan", (meta(FAR, 0, dtype=I32),)), ("tree_accept", accept_of(FAR, 1)),
+    ("tree_attention", attention_of(FAR, 1, 1, 1, 1, 4)), ("tree_attention", attention_of(1, 1, FAR, 1, 1, 4)), ("tree_attention", attention_of(1, 1, 1, 1, 1, FAR)),
+    ("tree_commit", commit_of(FAR, 1, 1, 1, 1, 4)), ("tree_commit", commit_of(1, FAR, 1, 1, 1, 4)), ("tree_commit", commit_of(1, 1, 1, FAR, 1, 4)),
+    ("tree_commit", commit_of(1, 1, 1, 1, FAR, 4)), ("tree_commit", commit_of(1, 1, 1, 1, 1, FAR)),
+    ("token_scores", (meta(1, FAR),)), ("token_scores", (meta(FAR, 5),)), ("token_scores", (meta(1, 5), meta(1, FAR, dtype=I32))),
+    ("quantize_rows_i8", (meta(FAR, 2),)), ("linear_i8", (meta(1, 2), meta(FAR, 2, dtype=torch.int8), meta(FAR))), ("linear_i8", (meta(FAR, 2), meta(1, 2, dtype=torch.int8), meta(1))),
+], ids=lambda a: a if isinstance(a, str) else "x".join("-".join(map(str, t.shape)) for t in a[:1]))
+def test_sizes_beyond_31_bits_are_refused(call, args):
+    """The library counts sizes in 32 bits: a larger one is refused, never cut to its low bits."""
+    with pytest.raises(ValueError, match=f"{call}: .*2\\^31"):
+        getattr(ops, call)(*args)

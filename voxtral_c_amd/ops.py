@@ -75,6 +75,13 @@ def _table(who, name, t, shape, dtype=_I32):
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _sizes(who, *tensors):
+    """The library counts sizes in 32 bits, and ctypes would hand it the low ones of a larger number without a word."""
+    for t in tensors:
+        if max(t.shape, default=0) > 0x7fffffff:
+            raise ValueError(f"{who}: shape {tuple(t.shape)}: sizes of 2^31 and more are not supported")
+
+
 def _device(who, *tensors):
     """The tensors' one GPU, as its number."""
     d = tensors[0].get_device()
@@ -110,6 +117,7 @@ def tree_plan(parents, n_nodes=None):
     if done is not None:
         return done
     who = "tree_plan"
+    _sizes(who, parents)
     _nodes(who, parents.shape)
     B, T = parents.shape if parents.dim() == 2 else (-1, -1)
     parents = _table(who, "parents", parents, (B, T))
@@ -132,6 +140,7 @@ def tree_attention(q, k, v, k_cache, v_cache, cache_len, ancestors, depth, scale
     if done is not None:
         return done
     who = "tree_attention"
+    _sizes(who, q, k, k_cache)
     if q.dim() != 4 or k_cache.dim() != 4 or k.dim() != 4:
         raise ValueError(f"{who}: q, k and the caches have 4 dimensions: got {q.dim()}, {k.dim()}, {k_cache.dim()}")
     B, T, H, D = q.shape
@@ -165,6 +174,7 @@ def tree_accept(tokens, choices, root_choice, parents, ancestors, depth, cache_l
     if done is not None:
         return done
     who = "tree_accept"
+    _sizes(who, tokens)
     _nodes(who, tokens.shape)
     B, T = tokens.shape if tokens.dim() == 2 else (-1, -1)
     if T == 0:
@@ -190,6 +200,7 @@ def tree_commit(k, v, k_cache, v_cache, path, n_accepted, cache_len):
         k, v, k_cache, v_cache = k[None], v[None], k_cache[None], v_cache[None]
     if _call.tree_commit(k, v, k_cache, v_cache, path, n_accepted, cache_len):
         return
+    _sizes(who, k, k_cache)
     if k.dim() != 5 or k_cache.dim() != 5:
         raise ValueError(f"{who}: k {tuple(k.shape)}, k_cache {tuple(k_cache.shape)}: [layers,] batch, rows, kv_heads, dim are needed")
     L, B, T, Hk, D = k.shape
@@ -220,6 +231,7 @@ def token_scores(logits, tokens=None, top=0):
     if done is not None:
         return TokenScores(*done)
     who = "token_scores"
+    _sizes(who, logits, *(() if tokens is None else (tokens,)))
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"{who}: logits have the shape {tuple(logits.shape)}: [rows, vocab] is needed")
     R, V = logits.shape
@@ -250,6 +262,7 @@ def quantize_rows_i8(x):
     if done is not None:
         return done
     who = "quantize_rows_i8"
+    _sizes(who, x)
     if x.dim() != 2 or not 1 <= x.shape[1] <= 131072:
         raise ValueError(f"{who}: x has the shape {tuple(x.shape)}: [rows, K] with K of 1 to 131072 is needed")
     number = _float_args(who, "x", x, x.shape)
@@ -267,6 +280,7 @@ def linear_i8(x, w, w_scale, bias=None):
     if done is not None:
         return done
     who = "linear_i8"
+    _sizes(who, x, w)
     if x.dim() != 2 or not 1 <= x.shape[1] <= 131072 or w.dim() != 2:
         raise ValueError(f"{who}: x has the shape {tuple(x.shape)}, w {tuple(w.shape)}: [rows, K] and [outputs, K] with K of 1 to 131072 are needed")
     M, K = x.shape
