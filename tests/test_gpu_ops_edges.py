@@ -87,3 +87,21 @@ def test_token_scores_rising_steps_of_large_numbers(V):
     assert abs(float(g.lse[0]) - lse) <= tol + 3 * e * 15 and abs(float(g.entropy[0]) - entropy) <= tol * (2 + entropy) * 2 + 3 * e * 15
     assert abs(float(g.logprob[0, 0]) - (5 - lse)) <= tol + 3 * e * 15 and g.top_index[:, 0].tolist() == [V - 1, V // 2]
     assert float(g.lse[1]) == torch.finfo(F32).max and float(g.entropy[1]) == 0 and float(g.logprob[1, 0]) == 0
+
+
+# ---- derivatives ---------------------------------------------------------------------------------------------------------------
+def test_forward_mode_tangents_are_refused_on_the_gpu():
+    """The compiled calls hand dual tensors back, and the Python ones refuse them; their primal values are ordinary tensors."""
+    from torch.autograd.forward_ad import dual_level, make_dual, unpack_dual
+    x, w, s = torch.randn(3, 32, device=DEV), torch.ones(5, 32, dtype=torch.int8, device=DEV), torch.ones(5, device=DEV)
+    plain = ops.linear_i8(x, w, s)
+    with dual_level():
+        d, ds = make_dual(x, torch.ones_like(x)), make_dual(s, torch.ones_like(s))
+        for f, args in ((ops.linear_i8, (d, w, s)), (ops.linear_i8, (x, w, ds)), (ops.linear_i8, (x, w, s, ds)), (ops.quantize_rows_i8, (d,)), (ops.token_scores, (d,)),
+                        (ops.token_scores, (d[:, 1:], None, 2))):
+            with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+                f(*args)
+        assert ops._call.linear_i8(d, w, s, None) is None and ops._call.quantize_rows_i8(d) is None and ops._call.linear_i8(x, w, s, None) is not None
+        assert torch.equal(ops.linear_i8(unpack_dual(d).primal, w, s), plain)
+        with torch.inference_mode():                                   # forward mode is off
+            assert torch.equal(ops.linear_i8(d, w, s), plain)

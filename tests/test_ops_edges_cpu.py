@@ -41,3 +41,27 @@ def test_sizes_beyond_31_bits_are_refused(call, args):
     """The library counts sizes in 32 bits: a larger one is refused, never cut to its low bits."""
     with pytest.raises(ValueError, match=f"{call}: .*2\\^31"):
         getattr(ops, call)(*args)
+
+
+def tangent(t):
+    return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+
+
+def test_forward_mode_tangents_are_refused():
+    """There are no derivatives in either direction: a dual tensor's tangent would be lost without a word."""
+    z = torch.zeros
+    x, w, s, q, k, c = z(2, 8), z(3, 8, dtype=torch.int8), z(3), z(1, 2, 2, 4), z(1, 2, 1, 4), z(1, 5, 1, 4)
+    n, t, a = z(1, dtype=I32), z(1, 2, dtype=I32), z(1, 2, 1, dtype=torch.int64)
+    calls = [(ops.quantize_rows_i8, [x], [0]), (ops.linear_i8, [x, w, s, s], [0, 2, 3]), (ops.token_scores, [x], [0]), (ops.tree_attention, [q, k, k, c, c, n, a, t], [0, 1, 2, 3, 4]),
+             (ops.tree_commit, [k[None], k[None], c[None], c[None], t, n, n], [0, 1, 2, 3]), (ops.tree_commit, [k, k, c, c, t, n, n], [0, 1, 2, 3])]
+    for f, args, places in calls:
+        for i in places:
+            with torch.autograd.forward_ad.dual_level():
+                dual = [*args[:i], tangent(args[i]), *args[i + 1:]]
+                for mode in (torch.enable_grad, torch.no_grad):        # (no_grad does not switch forward mode off)
+                    with mode(), pytest.raises(ValueError, match="tangent"):
+                        f(*dual)
+                with torch.inference_mode(), pytest.raises(ValueError, match="a GPU is needed"):
+                    f(*dual)
+            with pytest.raises(ValueError, match="a GPU is needed"):
+                f(*args)

@@ -4,13 +4,13 @@
 //
 // Each function takes the arguments of its namesake in ops.py, checks that they are what it takes without further ado, allocates results
 // and scratch memory from torch's allocator and calls the C entry (include/vox_hip_ops.h).  Anything else (a wrong shape, a table that is not contiguous, a tensor
-// that needs gradients, an error of the C entry) gives None: ops.py then does the same call itself and says what is wrong.
+// that needs gradients or has a tangent, an error of the C entry) gives None: ops.py then does the same call itself and says what is wrong.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
 #include <ATen/Functions.h>
 #include <ATen/core/Tensor.h>
-#include <c10/core/GradMode.h>
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -51,15 +51,16 @@ bool all_tensors(PyObject *const *args, int n) {
 struct Call {
     int device = -1, dtype = -1;
     at::ScalarType type = at::ScalarType::Undefined;
-    const bool grad = c10::GradMode::is_enabled();
+    const bool grad = c10::AutogradState::get_tls_state().get_grad_mode(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
     bool ok = true;
+    bool plain(Arg t) const { return !(grad && t.requires_grad()) && !(forward && t._fw_grad(0).defined()); }      // no derivative is wanted
     bool here(Arg t) {
         if (!t.is_cuda() || t.layout() != at::kStrided || t.is_neg()) return ok = false;
         if (device < 0) device = t.get_device();
         return ok = ok && t.get_device() == device;
     }
     void table(Arg t, at::IntArrayRef shape, at::ScalarType want = at::kInt) {
-        ok = ok && here(t) && t.scalar_type() == want && t.sizes() == shape && t.is_contiguous() && !(grad && t.requires_grad());
+        ok = ok && here(t) && t.scalar_type() == want && t.sizes() == shape && t.is_contiguous() && plain(t);
     }
     void floats(Arg t, at::IntArrayRef shape) {
         if (!ok || !here(t)) return;
@@ -69,7 +70,7 @@ struct Call {
             dtype = s == at::kFloat ? VOX_F32 : s == at::kBFloat16 ? VOX_BF16 : VOX_F16;
             ok = s == at::kFloat || s == at::kBFloat16 || s == at::kHalf;
         }
-        ok = ok && s == type && t.sizes() == shape && (t.stride(-1) == 1 || t.size(-1) <= 1) && !(grad && t.requires_grad());
+        ok = ok && s == type && t.sizes() == shape && (t.stride(-1) == 1 || t.size(-1) <= 1) && plain(t);
     }
     void *stream() {
         PyObject *d = PyLong_FromLong(device);

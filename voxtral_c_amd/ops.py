@@ -13,13 +13,15 @@ A verification pass takes several drafted tokens through the decoder at once::
 Every function enqueues HIP kernels on torch's current stream of the tensors' device and returns without waiting; results and scratch
 memory come from torch's allocator, so the calls may be captured into a graph.  Types: float32, bfloat16, float16 (one for all of a
 call's tensors), int32 for lengths, tokens and tree tables, int64 for the 64-bit words of ancestor sets.  Wrong arguments raise
-ValueError, a failed launch raises VoxError.  There is no backward pass: tensors that need gradients are refused.
+ValueError, a failed launch raises VoxError.  There are no derivatives: tensors that need gradients, or carry a
+forward-mode tangent, are refused.
 """
 import ctypes as C
 import struct
 from collections import namedtuple
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import VoxError, _ops_call as _call, hip
 
@@ -50,12 +52,20 @@ def _error(who):
     raise VoxError(f"{who}: {hip.vox_hip_last_error().decode()}")
 
 
+def _derivatives(who, name, t):
+    """Refuses what a backward pass, or forward mode, would want a derivative of."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{who}: {name} needs gradients: there is no backward pass (use torch.no_grad())")
+    if torch._C._is_fwd_grad_enabled() and unpack_dual(t).tangent is not None:
+        raise ValueError(f"{who}: {name} has a tangent: there is no forward-mode derivative (use unpack_dual(..).primal)")
+
+
 def _float_args(who, *named):
     """`named`: name, tensor, shape, name, .. .  One floating type of _DTYPES, the given shapes, a contiguous last dimension; returns the type's number."""
-    dtype, grad = named[1].dtype, torch.is_grad_enabled()
+    dtype = named[1].dtype
     for i in range(0, len(named), 3):
         t, shape = named[i + 1], named[i + 2]
-        if t.dtype is not dtype or t.shape != shape or (t.stride(-1) != 1 and shape[-1] > 1) or (grad and t.requires_grad) or dtype not in _DTYPES:
+        if t.dtype is not dtype or t.shape != shape or (t.stride(-1) != 1 and shape[-1] > 1) or dtype not in _DTYPES:
             name = named[i]
             if dtype not in _DTYPES:
                 raise ValueError(f"{who}: {name} is {dtype}: float32, bfloat16 or float16 are supported")
@@ -63,9 +73,8 @@ def _float_args(who, *named):
                 raise ValueError(f"{who}: {name} is {t.dtype}, {named[0]} is {dtype}: one type is needed")
             if t.shape != shape:
                 raise ValueError(f"{who}: {name} has the shape {tuple(t.shape)}: {tuple(shape)} is needed")
-            if t.requires_grad and grad:
-                raise ValueError(f"{who}: {name} needs gradients: there is no backward pass (use torch.no_grad())")
             raise ValueError(f"{who}: the last dimension of {name} is not contiguous")
+        _derivatives(who, named[i], t)
     return _DTYPES[dtype]
 
 
@@ -289,8 +298,7 @@ def linear_i8(x, w, w_scale, bias=None):
     if w.dtype != torch.int8 or w.shape[1] != K or (w.stride(1) != 1 and K > 1):
         raise ValueError(f"{who}: w is {w.dtype} {tuple(w.shape)}: int8 {(N, K)} with contiguous rows is needed")
     w_scale = _table(who, "w_scale", w_scale, (N,), torch.float32)
-    if w_scale.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{who}: w_scale needs gradients: there is no backward pass (use torch.no_grad())")
+    _derivatives(who, "w_scale", w_scale)
     d = _device(who, x, w, w_scale, *(() if bias is None else (bias,)))
     y = x.new_empty((M, N))
     wp, wst = w.data_ptr(), w.stride(0)
