@@ -105,3 +105,17 @@ def test_forward_mode_tangents_are_refused_on_the_gpu():
         assert torch.equal(ops.linear_i8(unpack_dual(d).primal, w, s), plain)
         with torch.inference_mode():                                   # forward mode is off
             assert torch.equal(ops.linear_i8(d, w, s), plain)
+
+
+def test_lazily_negated_tensors_are_refused_on_the_gpu():
+    x, c = torch.randn(3, 32, device=DEV), torch.zeros(2, 9, 2, 16, device=DEV)
+    k, n = torch.randn(2, 3, 2, 16, device=DEV), torch.ones(2, dtype=I32, device=DEV)
+    path = torch.zeros(2, 3, dtype=I32, device=DEV)
+    for f, args in ((ops.quantize_rows_i8, (torch._neg_view(x),)), (ops.token_scores, (torch._neg_view(x),)), (ops.tree_commit, (k, k, torch._neg_view(c), c, path, n, n)),
+                    (ops.tree_plan, (torch._neg_view(path),))):
+        with pytest.raises(ValueError, match="negated"):
+            f(*args)
+    assert (c == 0).all()
+    q, s = ops.quantize_rows_i8(torch._neg_view(x).resolve_neg())
+    want = ops.quantize_rows_i8(x)
+    assert torch.equal(q, -want[0]) and torch.equal(s, want[1])

@@ -65,3 +65,18 @@ def test_forward_mode_tangents_are_refused():
                     f(*dual)
             with pytest.raises(ValueError, match="a GPU is needed"):
                 f(*args)
+
+
+def test_lazily_negated_tensors_are_refused():
+    """Such a tensor's memory holds the values with the other sign: it is not read (or, a cache, written) as it is."""
+    z = torch.zeros
+    x, w, s, q, k, c = z(2, 8), z(3, 8, dtype=torch.int8), z(3), z(1, 2, 2, 4), z(1, 2, 1, 4), z(1, 5, 1, 4)
+    n, t, a = z(1, dtype=I32), z(1, 2, dtype=I32), z(1, 2, 1, dtype=torch.int64)
+    calls = [(ops.quantize_rows_i8, [x]), (ops.linear_i8, [x, w, s, s]), (ops.token_scores, [x, z(2, 1, dtype=I32)]), (ops.tree_attention, [q, k, k, c, c, n, a, t]),
+             (ops.tree_commit, [k[None], k[None], c[None], c[None], t, n, n]), (ops.tree_commit, [k, k, c, c, t, n, n]), (ops.tree_plan, [t, n]), (ops.tree_accept, [t, t, n, t, a, t, n])]
+    for f, args in calls:
+        for i in range(len(args)):
+            with pytest.raises(ValueError, match="negated"):
+                f(*args[:i], torch._neg_view(args[i]), *args[i + 1:])
+            with pytest.raises(ValueError, match="a GPU is needed"):
+                f(*args[:i], torch._neg_view(args[i]).resolve_neg(), *args[i + 1:])

@@ -92,8 +92,11 @@ def _sizes(who, *tensors):
 
 
 def _device(who, *tensors):
-    """The tensors' one GPU, as its number."""
+    """The tensors' one GPU, as its number; all of a call's tensors are seen here, and what lies in their memory has to be their values."""
     d = tensors[0].get_device()
+    for t in tensors:
+        if t.is_neg():
+            raise ValueError(f"{who}: a tensor of the shape {tuple(t.shape)} is negated lazily (use resolve_neg())")
     for t in tensors:
         if t.get_device() != d or d < 0:
             raise ValueError(f"{who}: tensors on {tensors[0].device} and {t.device}: " + ("one device is needed" if t.device != tensors[0].device else
