@@ -1,7 +1,13 @@
 """CPU: what the draft-verification operators refuse at the edges of their arguments, and how they are built and loaded."""
+import os
+import shutil
+import subprocess
+import sys
+
 import pytest
 import torch
 
+from conftest import ROOT
 from voxtral_c_amd import ops
 
 I32 = torch.int32
@@ -80,3 +86,45 @@ def test_lazily_negated_tensors_are_refused():
                 f(*args[:i], torch._neg_view(args[i]), *args[i + 1:])
             with pytest.raises(ValueError, match="a GPU is needed"):
                 f(*args[:i], torch._neg_view(args[i]).resolve_neg(), *args[i + 1:])
+
+
+def make_plan(*settings, path=None):
+    """What `make all` would run from nothing."""
+    r = subprocess.run(["make", "-n", "-B", "all", *settings], cwd=os.path.join(ROOT, "voxtral_c_amd"), capture_output=True, text=True, env={**os.environ, **({"PATH": path} if path else {})})
+    assert r.returncode == 0, r.stderr
+    return r.stdout
+
+
+def test_the_libraries_build_without_python_or_torch(tmp_path):
+    """The compiled calls need this interpreter's headers and its torch; the libraries need hipcc and a C compiler, and `make all` ends with them where that is all there is."""
+    full = make_plan()
+    assert "-o libvoxhip.so" in full and "-o libvoxtral.so" in full and "-o _ops_call.so" in full
+    for tool in ("make", "sh"):
+        os.symlink(shutil.which(tool), tmp_path / tool)
+    for plan in (make_plan("TORCH="), make_plan("PYINC=/nowhere"), make_plan(path=str(tmp_path))):        # no torch, no headers, no python3 at all
+        assert "-o libvoxhip.so" in plan and "-o libvoxtral.so" in plan and "-o _ops_call.so" not in plan
+
+
+def test_the_operators_load_without_their_compiled_calls():
+    """Without the module (not built, or built for another torch) the same calls go over ctypes, checks and all, and a warning says so."""
+    code = """
+import sys, warnings
+sys.modules["voxtral_c_amd._ops_call"] = None                          # the import fails
+import torch
+with warnings.catch_warnings(record=True) as seen:
+    warnings.simplefilter("always")
+    from voxtral_c_amd import ops
+assert any("_ops_call" in str(w.message) for w in seen)
+t = torch.zeros(1, 3, dtype=torch.int32)
+for call in (lambda: ops.tree_plan(t), lambda: ops.quantize_rows_i8(torch.zeros(2, 3)), lambda: ops.token_scores(torch.zeros(2, 3)),
+             lambda: ops.linear_i8(torch.zeros(2, 3), torch.zeros(4, 3, dtype=torch.int8), torch.zeros(4))):
+    try:
+        call()
+    except ValueError as e:
+        assert "a GPU is needed" in str(e)
+    else:
+        raise AssertionError
+print("fine")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
+    assert r.stdout.strip() == "fine", r.stderr

@@ -18,12 +18,23 @@ forward-mode tangent, are refused.
 """
 import ctypes as C
 import struct
+import warnings
 from collections import namedtuple
 
 import torch
 from torch.autograd.forward_ad import unpack_dual
 
-from . import VoxError, _ops_call as _call, hip
+from . import VoxError, hip
+
+try:
+    from . import _ops_call as _call
+except ImportError as e:                                               # not built, or built for another interpreter or torch
+    warnings.warn(f"{e}: the operators' calls go over ctypes (the same kernels, more host time per call)", RuntimeWarning, stacklevel=2)
+
+    class _call:
+        """Takes nothing: every call is made here."""
+
+        tree_plan = tree_attention = tree_accept = tree_commit = token_scores = quantize_rows_i8 = linear_i8 = bind = staticmethod(lambda *args: None)
 
 MAX_NODES = 256
 MAX_TOP = 64
