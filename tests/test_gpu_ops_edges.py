@@ -119,3 +119,27 @@ def test_lazily_negated_tensors_are_refused_on_the_gpu():
     q, s = ops.quantize_rows_i8(torch._neg_view(x).resolve_neg())
     want = ops.quantize_rows_i8(x)
     assert torch.equal(q, -want[0]) and torch.equal(s, want[1])
+
+
+# ---- caches that autograd holds ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("compiled", [True, False])
+def test_tree_commit_counts_as_a_write_of_the_caches(compiled, monkeypatch):
+    """A cache that a backward pass still needs cannot be written under it without a word: commits raise the tensors' version like torch's own in-place operations."""
+    if not compiled:
+        monkeypatch.setattr(ops, "_call", type("None_", (), {"__getattr__": lambda self, name: lambda *args: None})())
+    k, path, n = torch.randn(2, 3, 2, 16, device=DEV), torch.zeros(2, 3, dtype=I32, device=DEV), torch.ones(2, dtype=I32, device=DEV)
+    kc, vc = torch.zeros(2, 9, 2, 16, device=DEV), torch.zeros(2, 9, 2, 16, device=DEV)
+    q = torch.ones(16, device=DEV, requires_grad=True)
+    s = (kc * q).sum() + (vc[1] * q).sum()
+    before = kc._version, vc._version, k._version
+    ops.tree_commit(k, k, kc, vc, path, n, n)
+    assert (kc._version, vc._version, k._version) == (before[0] + 1, before[1] + 1, before[2])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        s.backward()
+    ops.tree_commit(k[None], k[None], kc[None], vc[None], path, n, n)
+    assert kc._version == before[0] + 2
+    with torch.inference_mode():                                       # tensors without a version, in and out of the mode
+        kc, vc = torch.zeros(2, 9, 2, 16, device=DEV), torch.zeros(2, 9, 2, 16, device=DEV)
+        ops.tree_commit(k, k, kc, vc, path, n, n)
+    ops.tree_commit(k, k, kc, vc, path, n, n * 0)
+    assert torch.equal(kc[:, 1], k[:, 0]) and torch.equal(kc, vc)

@@ -205,6 +205,8 @@ PyObject *tree_commit(PyObject *, PyObject *const *args, Py_ssize_t count) {
     OR_NONE(c.ok);
     OR_NONE(entry.tree_commit(c.dtype, (int)L, (int)B, (int)T, (int)Hk, (int)D, (int)cap, ptr(k), st[0], ptr(tensor(args[1])), st[1], ptr(kc), st[2], ptr(tensor(args[3])), st[3],
                               ints(tensor(args[4])), ints(tensor(args[5])), ints(tensor(args[6])), c.device, c.stream()) == 0);
+    for (int i : {2, 3})                                     // what autograd has saved of them is theirs no longer
+        if (!tensor(args[i]).is_inference()) tensor(args[i]).unsafeGetTensorImpl()->bump_version();
     Py_RETURN_TRUE;
     END
 }

@@ -217,7 +217,7 @@ def tree_accept(tokens, choices, root_choice, parents, ancestors, depth, cache_l
 
 def tree_commit(k, v, k_cache, v_cache, path, n_accepted, cache_len):
     """Files the path's keys and values into the ring caches, in place: k and v [layers, batch, nodes, kv_heads, dim], caches [layers, batch, cap,
-    kv_heads, dim] (or all four without the layers), cache_len the length before the path."""
+    kv_heads, dim] (or all four without the layers), cache_len the length before the path.  The caches' versions rise, as by torch's own in-place operations."""
     who = "tree_commit"
     if k.dim() == 4:
         k, v, k_cache, v_cache = k[None], v[None], k_cache[None], v_cache[None]
@@ -241,6 +241,9 @@ def tree_commit(k, v, k_cache, v_cache, path, n_accepted, cache_len):
                                k_cache.data_ptr(), _Strides(*k_cache.stride()[:4]), v_cache.data_ptr(), _Strides(*v_cache.stride()[:4]),
                                path.data_ptr(), n_accepted.data_ptr(), cache_len.data_ptr(), d, _stream(d)):
         _error(who)
+    for t in (k_cache, v_cache):                                       # what autograd has saved of them is theirs no longer
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
 
 
 TokenScores = namedtuple("TokenScores", "logprob entropy lse top_index top_logprob")
