@@ -5,6 +5,8 @@ import numpy as np
 import pytest
 import torch
 
+from test_gpu_ops import check_linear
+
 import voxtral_c_amd as v
 from voxtral_c_amd import ops
 
@@ -143,3 +145,17 @@ def test_tree_commit_counts_as_a_write_of_the_caches(compiled, monkeypatch):
         ops.tree_commit(k, k, kc, vc, path, n, n)
     ops.tree_commit(k, k, kc, vc, path, n, n * 0)
     assert torch.equal(kc[:, 1], k[:, 0]) and torch.equal(kc, vc)
+
+
+# ---- 8-bit integers: scales of very different sizes ----------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,K,N", [(1, 1280, 40), (20, 1280, 130), (25, 77, 65), (40, 1280, 129), (64, 5120, 256), (300, 1280, 140)])
+def test_linear_i8_scales_of_very_different_sizes(M, K, N, dtype):
+    """Outputs of ordinary size from rows of tiny numbers and a large weight scale, or the other way round: no intermediate product leaves f32's range."""
+    rng = np.random.default_rng(M + N)
+    w = torch.as_tensor(rng.integers(60, 128, (N, K)).astype(np.int8)).to(DEV)
+    x = torch.as_tensor((rng.random((M, K)) + 0.5).astype(np.float32)).to(DEV)
+    for x_size, w_size in ((2.0 ** -115, 2.0 ** 112), (2.0 ** 115, 2.0 ** -118), (2.0 ** -60, 2.0 ** 60)):
+        ws = torch.as_tensor((rng.random(N) + 0.5).astype(np.float32)).to(DEV) * w_size
+        y = check_linear((x * x_size).to(dtype), w, ws, None, dtype)
+        assert torch.isfinite(y).all() and (y > 1).all()

@@ -1,5 +1,6 @@
 // vox_linear_i8.h — products in 8-bit integers: y = x_scale * w_scale * (xq . w), one scale per row of x and per output channel.
 #pragma once
+#include <type_traits>
 #include "vox_ops_common.h"
 
 namespace vox {
@@ -75,8 +76,14 @@ struct LinearI8Args {
     int *part;                   // [splits, padded rows, padded channels]: sums of a part of K each, where K is split
     int splits;
 };
-// Three roundings of f32 (the sum's conversion and two products) and the one to the output's type; the sum itself is exact.
-__device__ __forceinline__ float i8_scaled(int acc, float xs, float ws) { return ((float)acc * ws) * xs; }
+// Three roundings of f32 (the sum's conversion and two products) and the one to the output's type; the sum itself is exact.  Where the first product
+// leaves f32's range the row's scale, which may be as small as 2^-126, goes first: if both orders overflow, so does the result.  The sum is at most 2^31:
+// no weight scale up to I8_SAFE does that, and `LARGE` may be false.
+constexpr float I8_SAFE = 0x1p96f;
+template <bool LARGE = true> __device__ __forceinline__ float i8_scaled(int acc, float xs, float ws) {
+    const float v = (float)acc, p = v * ws;
+    return LARGE && __builtin_isinf(p) ? v * xs * ws : p * xs;
+}
 template <typename T> __device__ __forceinline__ T i8_out(int acc, float xs, float ws, const T *bias, int n) {
     float v = i8_scaled(acc, xs, ws);
     if (bias) v += (float)bias[n];
@@ -331,23 +338,28 @@ template <typename T, int BM, int STAGES> __global__ __launch_bounds__(256) void
     // lane: row lane % 32 of a block, channels 8 g + 4 (lane / 32) + 0..3 in registers 4 g + 0..3
     constexpr int LD = I8_BN + 16 / sizeof(T);
     T *out = reinterpret_cast<T *>(lds);
+    auto scale = [&](auto is_large) {                        // (the question asked for each output costs 4 % of the kernel's time)
+        constexpr bool large = decltype(is_large)::value;
 #pragma unroll
-    for (int i = 0; i < MI; i++) {
-        const int row = wm * (BM / 2) + i * 32 + (lane & 31);
-        const float xs = sx[row];
+        for (int i = 0; i < MI; i++) {
+            const int row = wm * (BM / 2) + i * 32 + (lane & 31);
+            const float xs = sx[row];
 #pragma unroll
-        for (int j = 0; j < NJ; j++)
+            for (int j = 0; j < NJ; j++)
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                typedef T out4 __attribute__((ext_vector_type(4)));
-                const int ch = wn * 64 + j * 32 + g * 8 + (lane >> 5) * 4;
-                const f32x4 ws = *reinterpret_cast<const f32x4 *>(sw + ch), bias = *reinterpret_cast<const f32x4 *>(sb + ch);
-                out4 v;
+                for (int g = 0; g < 4; g++) {
+                    typedef T out4 __attribute__((ext_vector_type(4)));
+                    const int ch = wn * 64 + j * 32 + g * 8 + (lane >> 5) * 4;
+                    const f32x4 ws = *reinterpret_cast<const f32x4 *>(sw + ch), bias = *reinterpret_cast<const f32x4 *>(sb + ch);
+                    out4 v;
 #pragma unroll
-                for (int r = 0; r < 4; r++) v[r] = from_f32<T>(i8_scaled(acc[j][i][g * 4 + r], xs, ws[r]) + bias[r]);
-                *reinterpret_cast<out4 *>(out + row * LD + ch) = v;
-            }
-    }
+                    for (int r = 0; r < 4; r++) v[r] = from_f32<T>(i8_scaled<large>(acc[j][i][g * 4 + r], xs, ws[r]) + bias[r]);
+                    *reinterpret_cast<out4 *>(out + row * LD + ch) = v;
+                }
+        }
+    };
+    if (__any(!(fabsf(sw[wn * 64 + lane]) <= I8_SAFE))) scale(std::true_type{});      // (the wave's 64 channels)
+    else scale(std::false_type{});
     __syncthreads();
     const int rows = min(BM, a.M - m0), cols = min(I8_BN, a.N - n0);
     T *y = (T *)a.y + m0 * a.y_stride + n0;
