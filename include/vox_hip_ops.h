@@ -46,7 +46,7 @@ int vox_hip_tree_plan(const int32_t *parents, const int32_t *n_nodes, int batch,
  *   the cache's positions p of [max(0, cache_len - cap), cache_len) with window <= 0 or p > cache_len + depth[i] - window
  *   (position p lives in row p % cap of the ring), and
  *   the nodes j in ancestors[b, i] (any bit set, not only trees') with window <= 0 or depth[j] > depth[i] - window;
- * kv head = h / (heads / kv_heads).  scale is finite and not 0.  A row with depth -1 or with nothing to attend to gives zeros (lse = -inf); what masked keys and
+ * kv head = h / (heads / kv_heads).  scale is not 0 and at most 2e38 in size.  A row with depth -1 or with nothing to attend to gives zeros (lse = -inf); what masked keys and
  * values hold, NaN and infinities too, does not matter (one that a row does see may make the row's outputs infinite or NaN).  cache_len <= 0 is an empty cache.  Sums and softmax statistics are f32. */
 typedef struct vox_hip_tree_attn {
     const void *q, *k, *v;               /* [batch, nodes, heads | kv_heads, head_dim] */

@@ -128,3 +128,11 @@ print("fine")
 """
     r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
     assert r.stdout.strip() == "fine", r.stderr
+
+
+@pytest.mark.parametrize("scale,fine", [(1.0, True), (-1e38, True), (1e38, True), (3e38, False), (-2.5e38, False), (0.0, False), (float("inf"), False), (float("nan"), False), (1e-30, True)])
+def test_tree_attention_takes_scales_whose_base_2_form_is_finite(scale, fine):
+    """The softmax runs in base 2: scale * log2(e) has to be a number, or a score of 0 would become NaN."""
+    args = ops._ATTN.pack(*[4096] * 10, *[8] * 18, 0, 1, 2, 4, 2, 64, 8, 0, scale, 0)
+    assert (ops.hip.vox_hip_tree_attention_workspace(args) >= 0) == fine
+    assert fine or "scale" in ops.hip.vox_hip_last_error().decode()

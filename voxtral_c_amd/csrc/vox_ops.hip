@@ -137,7 +137,7 @@ int check_attn(const vox_hip_tree_attn_t *a) {
     CHECK(a->kv_heads >= 1 && a->heads >= 1 && a->heads <= 4096 && a->heads % a->kv_heads == 0, "%s: %d heads over %d kv heads", who, a->heads, a->kv_heads);
     CHECK(a->head_dim >= 1 && a->head_dim <= TREE_SCALAR_MAX_D, "%s: head_dim %d (at most %d)", who, a->head_dim, TREE_SCALAR_MAX_D);
     CHECK(a->cap >= 1, "%s: a cache of %d rows", who, a->cap);
-    CHECK(a->scale != 0.f && a->scale - a->scale == 0.f, "%s: scale %g (a finite number other than 0)", who, (double)a->scale);
+    CHECK(a->scale != 0.f && a->scale >= -2e38f && a->scale <= 2e38f, "%s: scale %g (a finite number other than 0, of at most 2e38)", who, (double)a->scale);      // (times log2 e)
     CHECK(a->reserved == 0, "%s: reserved is not 0", who);
     return 0;
 }
