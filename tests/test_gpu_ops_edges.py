@@ -159,3 +159,16 @@ def test_linear_i8_scales_of_very_different_sizes(M, K, N, dtype):
         ws = torch.as_tensor((rng.random(N) + 0.5).astype(np.float32)).to(DEV) * w_size
         y = check_linear((x * x_size).to(dtype), w, ws, None, dtype)
         assert torch.isfinite(y).all() and (y > 1).all()
+
+
+# ---- errors of others ----------------------------------------------------------------------------------------------------------
+def test_an_earlier_error_of_another_call_is_not_this_calls():
+    """A HIP call of the same thread that failed before (asking for a device that is not there) does not make a launch fail that succeeds."""
+    parents, words, depth = torch.full((1, 3), -1, dtype=I32, device=DEV), torch.zeros(1, 3, 1, dtype=torch.int64, device=DEV), torch.full((1, 3), 7, dtype=I32, device=DEV)
+    torch.cuda.synchronize()
+    assert v.hip.hipSetDevice(1000) != 0 and v.hip.hipPeekAtLastError() != 0
+    try:
+        assert v.hip.vox_hip_tree_plan(parents.data_ptr(), None, 1, 3, words.data_ptr(), depth.data_ptr(), 0, torch.cuda.current_stream().cuda_stream) == 0, v.hip.vox_hip_last_error()
+    finally:
+        v.hip.hipGetLastError()
+    assert depth.tolist() == [[0, 0, 0]]

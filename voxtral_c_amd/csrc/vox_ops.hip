@@ -46,6 +46,7 @@ struct OnDevice {
         }
         if (k != 1) { refuse("%s: device %d is not gfx950: these kernels are written for MI355X only", who, dev); return; }
         if (before != dev && hipSetDevice(dev) != hipSuccess) { (void)hipGetLastError(); refuse("%s: hipSetDevice(%d) failed", who, dev); return; }
+        (void)hipGetLastError();                             // an earlier call's error is not this launch's (launched() asks the thread's last one)
         ok = true;
     }
     ~OnDevice() { if (ok && before != device) (void)hipSetDevice(before); }
