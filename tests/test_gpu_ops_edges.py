@@ -172,3 +172,26 @@ def test_an_earlier_error_of_another_call_is_not_this_calls():
     finally:
         v.hip.hipGetLastError()
     assert depth.tolist() == [[0, 0, 0]]
+
+
+# ---- f32 products in parts -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("D", [4, 64, 128, 256])
+@pytest.mark.parametrize("T,G", [(2, 4), (40, 4), (40, 1), (70, 2)])
+def test_tree_attention_f32_numbers_whose_parts_are_all_as_large_as_can_be(T, G, D):
+    """Many f32 rows are multiplied as three bf16 parts per number, cut off and not rounded, and three of nine products are left out: at most 2^-21 of a
+    product.  Rows that see one key show it: the log-sum is the score, one product of two such numbers, and the output is the value."""
+    worst = 1 + 2.0 ** -7 - 2.0 ** -23
+    rng = np.random.default_rng(T + D)
+    sign = lambda *s: torch.as_tensor(rng.choice([-1.0, 1.0], s)).to(F32).to(DEV)  # noqa: E731
+    q = torch.zeros(1, T, G, D, device=DEV)
+    q[..., 1] = worst * 4
+    k, v_ = sign(1, T, 1, D) * worst, sign(1, T, 1, D) * worst * 2.0 ** torch.arange(-D // 2, D - D // 2, device=DEV).clamp(-60, 60)
+    alone, depth = ops.tree_plan(torch.full((1, T), -1, dtype=I32, device=DEV))
+    empty = torch.full((1, 8, 1, D), math.nan, device=DEV)
+    out, lse = ops.tree_attention(q, k, v_, empty, empty, torch.zeros(1, dtype=I32, device=DEV), alone, depth, scale=0.75, return_lse=True)
+    # the weight is e^(score - maximum) of a maximum that was rounded, so near 1 and not 1; (weight value) / weight: 2^-21 left out, the six products' sum
+    # 6 e, the quotient e
+    assert bool(((out.double() / v_.double() - 1).abs() <= 2.0 ** -21 + 7 * 2.0 ** -24).all())
+    want = (q[..., 1].double() * k[..., 1].double() * 0.75).cpu().numpy()
+    # left out: 2^-21; the six products' sum: 6 e; the scale and its way to base 2 and back (two constants, three products): 5 e
+    assert (np.abs(lse.cpu().double().numpy() / want - 1) <= 2.0 ** -21 + 11 * 2.0 ** -24).all()

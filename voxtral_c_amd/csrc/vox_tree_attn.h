@@ -25,7 +25,9 @@ __device__ __forceinline__ void tree_range(const TreeAttnArgs &a, int b, int64_t
 }
 
 // One workgroup of four waves per (node, head, sequence): a wave takes every fourth key, its lanes split the head's dimensions, and the
-// waves' (max, sum, output) are joined at the end.  Any head_dim up to 256, any stride and alignment; a key that is masked is never read.
+// waves' (max, sum, output) are joined at the end.  Any head_dim up to 256, any stride and alignment; a key that is masked is never read.  Bound by the latency
+// of one key after another, each read again for every node and head: 2 nodes x 32 heads of 33 dimensions over 8192 keys, f32: 1.56 ms; 4 x 4 nodes x 32 heads of
+// 100, bf16: 3.4 ms, where 104 dimensions (rows of whole 16-byte loads) take 37 us.  It is there so that every layout is answered, not for speed.
 constexpr int TREE_SCALAR_MAX_D = 256;
 template <typename T> __global__ __launch_bounds__(256) void k_tree_attn_scalar(TreeAttnArgs a) {
     __shared__ float sm[4], sl[4], so[4][TREE_SCALAR_MAX_D];
@@ -101,8 +103,10 @@ template <typename T> __global__ __launch_bounds__(256) void k_tree_attn_scalar(
 //            the read of the cache, and for short caches by latency: 2 nodes x 4 heads over 232 keys, f32: 11.2 us, the join of 4 parts 3.9 us.
 //   shared   (more rows) the four waves have rows of their own and share the steps' keys in LDS, which global_load_lds fills STAGES steps ahead:
 //            nothing of it is in registers, and the cache is read once per 64 or 128 rows.  24 nodes x 4 heads over 4 x 40000 keys, bf16: 127 us for 557 MB
-//            (4.4 TB/s), bound by the read; 64 nodes x 4 heads over 2 x 8191 keys, f32: 175 us, bound by the vector unit, which splits the numbers (below).
+//            (4.4 TB/s), bound by the read; 64 nodes x 4 heads over 2 x 8191 keys, f32: 174 us, bound by the vector unit, which splits the numbers (below).
 // Where both would do, 32 rows of 128 dimensions over 4 x 16000 keys: own 78 us, shared 57 in bf16, 152 and 125 in f32.
+// Head sizes between 64, 128 and 256 run as the next one of these, and none of their tiles is plain (below): 96 dimensions, 24 nodes x 4 heads over 4 x 40000
+// keys, bf16: 130 us for 418 MB, 3.2 TB/s; 2 nodes x 4 heads: 97 us, 4.3 TB/s (128 dimensions: 115 us, 4.9 TB/s).
 // Each wave runs its own online softmax (one maximum and sum per row); waves with different keys are joined through LDS at the end, the parts of a
 // long cache by k_tree_attn_join.
 template <typename T> struct AttnType;
@@ -130,10 +134,13 @@ template <> struct AttnType<f16_t> {
 };
 
 constexpr int ATTN_WAVES = 4;
-// Shared keys of f32 are multiplied on the bf16 pipe: a number is exactly the sum of three bf16 ones (8 of its 24 bits each), and of the nine
-// products the six down to 2^-16 of the largest are taken, the rest is below 2^-24.  An f32 matrix instruction takes the vector unit's cycles (measured:
+// Shared keys of f32 are multiplied on the bf16 pipe: a number is exactly the sum of three bf16 ones (8 of its 24 bits each, cut off, so all of its sign),
+// and of the nine products six are taken.  With the leading bit as 1 the middle part is below 2^-7 and the low one below 2^-15: the two products of a
+// middle and a low part that are left out are up to 2^-21 of the whole product together (2^-21.03 for 1 + 2^-7 - 2^-23 squared; 2^-24.5 on average
+// over normally distributed numbers), always with its sign.  An f32 matrix instruction takes the vector unit's cycles (measured:
 // the two run one after the other, 0.23 + 0.23 ms -> 0.46 ms), a bf16 one does not, and six of them take 6 x 17 cycles where f32 takes 8 x 33:
-// 64 rows over 4 x 16000 keys 163 -> 142 us, 32 rows 152 -> 125.  Splitting each key once per workgroup into LDS instead of in every wave was slower (178 us).
+// 64 rows over 4 x 16000 keys 163 -> 142 us, 32 rows 152 -> 125.  Splitting each key once per workgroup into LDS, by eight waves in step, was slower at
+// 64 rows (178 us instead of 142) and faster above (128 rows 239 instead of 267, 256 rows 432 instead of 481); there is one form for all of them.
 template <typename T, bool SHARED> constexpr bool ATTN_SPLIT = SHARED && sizeof(T) == 4;
 template <typename T, bool SHARED> constexpr int ATTN_KT = SHARED || sizeof(T) == 2 ? 32 : 16;              // keys of a step
 template <typename T> constexpr int ATTN_STAGES = sizeof(T) == 4 ? 2 : 3;                                   // (two workgroups per CU)
