@@ -30,7 +30,7 @@ __device__ __forceinline__ RowScale row_scale(unsigned amax_bits) {
 
 // One workgroup per row: q [rows, ldq] (columns K .. ldq - 1 are zeros), scale [rows].  Bound by the row's two trips (the second one hits the
 // caches; keeping the row in registers instead measured the same) and, for few rows, by their latency: as many threads as give each one load, up to 1024
-// (25 x 5120 bf16: 3.9 us, with 256 threads 5.2).  4099 x 1280 bf16: 8.5 us.  N elements per load: K, stride and x allow it, and ldq % N = 0.
+// (25 x 5120 bf16: 3.9 us, with 256 threads 5.2).  4099 x 1280 bf16: 6.8 us on its own, 8.6 - 10 between products, for 15.7 MB.  N elements per load: K, stride and x allow it, and ldq % N = 0.
 constexpr int I8_QUANT_THREADS = 1024;
 template <typename T, int N> __global__ __launch_bounds__(I8_QUANT_THREADS) void k_quant_rows_i8(const T *x, int64_t stride, int K, int ldq, int8_t *q, float *scale) {
     __shared__ unsigned red[I8_QUANT_THREADS / 64];
@@ -90,7 +90,9 @@ template <typename T> __device__ __forceinline__ T i8_out(int acc, float xs, flo
     return from_f32<T>(v);
 }
 
-// Any K, stride and alignment: 64 x 64 outputs per workgroup, slices of 64 bytes of K through LDS byte by byte, v_dot4 products.
+// Any K, stride and alignment: 64 x 64 outputs per workgroup, slices of 64 bytes of K through LDS byte by byte, v_dot4 products.  Bound by the byte loads:
+// 25 x 1283 x 6144 takes 123 us (K 1280: 9), 400 rows 153 (17).  It is there so that every layout is answered; a weight matrix laid out once can have
+// rows of whole 16 bytes.
 template <typename T> __global__ __launch_bounds__(256) void k_linear_i8_bytes(LinearI8Args a) {
     __shared__ int xs[64][17], ws[64][17];
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
@@ -123,8 +125,8 @@ template <typename T> __global__ __launch_bounds__(256) void k_linear_i8_bytes(L
 // ---- few rows: a read of the weights --------------------------------------------------------------------------------------------
 // A workgroup makes 16 output channels of MT x 16 rows; its waves split K and their whole-number sums are added through LDS (exact in any order).
 // v_mfma_i32_16x16x64_i8 with the weights as A operand: lane = (channel lane % 16, 16 bytes of K), loaded straight from the row-major matrix, 64 bytes of
-// each of 16 rows per instruction and two neighbouring instructions per 128-byte line.  25 x 5120 x 1280: 8.5 us, 0.8 TB/s of weights (80 workgroups; operands
-// four steps ahead changed nothing), 11.4 us a call with the quantiser's launch.
+// each of 16 rows per instruction and two neighbouring instructions per 128-byte line.  25 x 5120 x 1280: 8.6 us, 0.8 TB/s of weights (80 workgroups; operands
+// four steps ahead changed nothing), 11.7 us a call with the quantiser's launch.
 constexpr int I8_ROWS_WAVES = 8;
 template <typename T, int MT> __global__ __launch_bounds__(64 * I8_ROWS_WAVES) void k_linear_i8_rows(LinearI8Args a) {
     __shared__ i32x4 part[I8_ROWS_WAVES][MT][64];
@@ -163,7 +165,7 @@ template <typename T, int MT> __global__ __launch_bounds__(64 * I8_ROWS_WAVES) v
 
 // The same in one launch for a few rows (single tokens): every workgroup quantises all of x into its LDS while its first weights are on their way.  Up
 // to I8_FEW elements of x: 32 per thread, about a microsecond; a launch of its own costs 3 us (1 x 1280 x 6144,
-// f32: 13.9 -> 10.9 us a call then, 5.8 now; 1.4 TB/s of weights).
+// f32: 13.9 -> 10.9 us a call then; now 6.5 with weights from memory, 1.2 TB/s, and 5.8 with the same ones again and again).
 constexpr int I8_FEW = 16384, I8_FEW_ROWS = 16, I8_FEW_AHEAD = 2;
 template <typename T, int N> __global__ __launch_bounds__(64 * I8_ROWS_WAVES) void k_linear_i8_few(LinearI8Args a, const T *x, int64_t x_stride) {
     __shared__ i32x4 part[I8_ROWS_WAVES][64];
@@ -230,7 +232,8 @@ template <typename T, int N> __global__ __launch_bounds__(64 * I8_ROWS_WAVES) vo
 // go from memory into LDS without registers (global_load_lds_dwordx4: a wave's instruction brings 128 bytes of each of 8 rows), STAGES of them in
 // flight with one barrier per slice.  16-byte pieces of a row are stored at (piece ^ (row / 2 % 8)): of the MFMA operand reads (lane = row, one
 // piece) 16 lanes at a time then touch every one of the 64 banks once (with row % 8 the counters show a conflict on every second cycle).  Outputs leave through LDS so that rows are written in whole lines.
-// 4099 x 1280 x 10240: 82 us, 1.3 POP/s (31 % of the pipe's cycles; 84 MB of the output alone take 18 us); 8192^3: 1.6 POP/s.  What bounds it is neither LDS nor
+// 4099 x 1280 x 10240 bf16: 82 - 86 us, 1.3 POP/s (31 % of the pipe's cycles; 84 MB of the output alone take 18 us; 96 in a run of
+// 60 under the profiler); 8192^3: 1.6 POP/s.  What bounds it is neither LDS nor
 // the depth of the pipeline: 256 x 128 tiles with slices of 64 bytes, three stages and a quarter less traffic per product took 107 us where these took 103,
 // 256 x 128 with three stages and one workgroup per CU 119.
 constexpr int I8_BN = 128, I8_BK = 128;

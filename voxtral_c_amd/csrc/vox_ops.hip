@@ -159,8 +159,9 @@ bool attn_wide(const vox_hip_tree_attn_t *a) {
     return a->head_dim % unit == 0;
 }
 // Up to 16 rows (nodes x heads of a kv head; 32 where a head has up to 64 dimensions) the waves of a workgroup have keys of their own, above that
-// rows of their own (64 or 128 per workgroup) and shared keys (32 rows of 128 dimensions over 4 x 16000 keys: own 78 us, shared 57 in bf16; 152 and 125
-// in f32).  Splits: enough workgroups for two per CU, but at least one key tile per wave in each.
+// rows of their own (64 or 128 per workgroup) and shared keys.  32 rows of 128 dimensions over 4 x 16000 keys: own 78 us, shared 57 in bf16; 152 and 125
+// in f32.  64 dimensions, 4 x 16000 keys, own / shared: f32 32 rows 58 / 73 us, 36 rows 91 / 74; bf16 32 rows 36 / 33, 36 rows 45 / 34; over 8 x 1000 keys
+// the two are within 10 % of each other.  Splits: enough workgroups for two per CU, but at least one key tile per wave in each.
 struct AttnLaunch { bool wide, shared; int DP, RT, row_blocks, key_waves, splits; int64_t ws; };
 AttnLaunch attn_launch(const vox_hip_tree_attn_t *a) {
     AttnLaunch l{};
@@ -309,7 +310,8 @@ template <typename T> void launch_quant(const T *x, int64_t stride, int64_t rows
 }
 // Up to 32 rows the product is a read of the weights (k_linear_i8_rows).  Above, tiles of 128 rows x 128 channels, of 64 rows where there would be
 // fewer than 192; K is split where even those are fewer than 100, into parts of six slices of 128 or more: the parts' way through memory and
-// the third launch cost 6 - 9 us (64 x 5120 x 1280: 20.7 -> 17.3 us; 256 x 5120 x 5120, 160 tiles: 28.7 us whole, 31.7 split).
+// the third launch cost 6 - 9 us.  Whole / split: K 5120, 10 tiles 24.3 / 16.2 us, 40 tiles 25.3 / 18.7, 80 tiles 25.7 / 20.8, 120 tiles 27.3 / 24.3 (the limit
+// leaves these whole), 160 tiles 28.7 / 31.7; K 2560, 80 tiles 16.9 / 18.7 (and splits these).
 struct I8Plan { bool few; int BM, tiles_m, tiles_n, splits; int64_t scale_at, part_at, ws; };
 I8Plan i8_plan(int64_t rows, int K, int N, bool wide) {
     I8Plan p{};

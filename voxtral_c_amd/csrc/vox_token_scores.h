@@ -2,9 +2,11 @@
 //
 // Bound by reading the logits once.  A thread keeps the running maximum and sums of its elements, a wave keeps the `top` largest
 // elements of its share as a sorted list with one entry per lane, and both are joined over lanes, waves and (few long rows) parts of a row.
-// Measured, vocabulary 131072, logits read once in a call: 386 rows of f32, top 4: 49 us (4.1 TB/s; the kernel 43 us, 4.7 TB/s, joining the parts
-// 6 us); 1501 rows of bf16, top 32: 100 us (3.9 TB/s: a bf16 logit costs the same vector work as an f32 one at half the bytes, and here both count).
-// One row, top 8: 7.7 + 5.1 us for parts and join, bound by latency; 12 us a call from Python.
+// Measured, vocabulary 131072, on rows that no cache holds: 386 rows of f32, top 4: 49 us (4.1 TB/s; the kernel 43 us, 4.7 TB/s, joining the parts
+// 6 us); 1501 rows top 32: bf16 100 us, f16 101 (3.9 TB/s: a 16-bit logit costs the same vector work as an f32 one at half the bytes, and here both count).
+// One row, top 8: 7.0 + 5.2 us for parts and join, bound by latency; 12 us a call from Python.
+// Rows that do not start on 16 bytes (a contiguous vocabulary that is no multiple of 16 bytes) are read one element per load: 1501 rows of 131071 bf16
+// logits 147 us instead of 100, 386 of 131071 f32 63 instead of 49, one row 17 instead of 12.
 #pragma once
 #include "vox_ops_common.h"
 
