@@ -161,7 +161,8 @@ int64_t vox_hip_adapter_rows(const vox_hip_engine_t *e);
 /* Device pointer of the adapter ring (for RCCL/torch interop) and its row capacity. */
 void *vox_hip_adapter_devptr(vox_hip_engine_t *e, int64_t *cap_rows);
 /* Device pointers of a decoder layer's K and V rings, [cap_rows, dec_kv_heads, dec_head_dim] f32, position p in row p % cap_rows (the
- * caches of the operators in vox_hip_ops.h; reference: kv_cache_k / kv_cache_v, voxtral.h:154-204). */
+ * caches of the operators in vox_hip_ops.h; reference: kv_cache_k / kv_cache_v, voxtral.h:154-204).  They live as long as the engine; its own work on
+ * them runs on its stream, and rows written from outside do not move vox_hip_decoder_kv_len: the engine's next steps write over them. */
 int vox_hip_decoder_kv_devptr(vox_hip_engine_t *e, int layer, void **k, void **v, int *cap_rows);
 
 /* ---- multi-GPU encoder sharding (exact context parallelism) ------

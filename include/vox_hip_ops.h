@@ -47,7 +47,11 @@ int vox_hip_tree_plan(const int32_t *parents, const int32_t *n_nodes, int batch,
  *   (position p lives in row p % cap of the ring), and
  *   the nodes j in ancestors[b, i] (any bit set, not only trees') with window <= 0 or depth[j] > depth[i] - window;
  * kv head = h / (heads / kv_heads).  scale is not 0 and at most 2e38 in size.  A row with depth -1 or with nothing to attend to gives zeros (lse = -inf); what masked keys and
- * values hold, NaN and infinities too, does not matter (one that a row does see may make the row's outputs infinite or NaN).  cache_len <= 0 is an empty cache.  Sums and softmax statistics are f32. */
+ * values hold, NaN and infinities too, does not matter (one that a row does see may make the row's outputs infinite or NaN).  cache_len <= 0 is an empty cache.
+ * Arithmetic: scores, softmax statistics and sums are f32.  bf16 and f16: every weight p_j is rounded to that type in front of its product with v (half
+ * a step: 2^-8 or 2^-11 of the weighted mean of |v|), their sum is taken of the unrounded ones.  f32: where a kv head has many rows, products are taken
+ * in bf16 parts and are up to 2^-21 of themselves too small.  The outputs' sums run before the division by the weights' sum: values of more than 1e28 may
+ * overflow on the way. */
 typedef struct vox_hip_tree_attn {
     const void *q, *k, *v;               /* [batch, nodes, heads | kv_heads, head_dim] */
     const void *k_cache, *v_cache;       /* [batch, cap, kv_heads, head_dim] */
@@ -85,7 +89,8 @@ int vox_hip_tree_commit(int dtype, int layers, int batch, int nodes, int kv_head
  * the `top` largest logits' indexes and log probabilities [rows, top], equal logits by the lowest index.  given = 0 / top = 0: those
  * pointers may be NULL.  A logit of -inf is a token of probability 0 (a row of nothing else: lse -inf, entropy 0, every logprob -inf);
  * a NaN makes its row's lse, entropy and logprobs NaN and counts as the largest; +inf without a NaN makes lse +inf and
- * the entropy and log probabilities NaN. */
+ * the entropy and log probabilities NaN.  Finite logits of any size are ordinary ones (tokens switched off with the type's lowest number as well).  Sums
+ * are f32. */
 int64_t vox_hip_token_scores_workspace(int dtype, int64_t rows, int vocab, int top);
 int vox_hip_token_scores(int dtype, const void *logits, int64_t row_stride, int64_t rows, int vocab, const int32_t *tokens, int given, int top,
                          float *logprob, float *entropy, float *lse, int32_t *top_index, float *top_logprob, void *ws, size_t ws_bytes,
@@ -96,8 +101,8 @@ int vox_hip_token_scores(int dtype, const void *logits, int64_t row_stride, int6
 int vox_hip_quantize_rows_i8(int dtype, const void *x, int64_t row_stride, int64_t rows, int K, int8_t *q, float *scale, int device, void *stream);
 
 /* y[m, n] = x_scale[m] * w_scale[n] * sum_k xq[m, k] * w[n, k] (+ bias[n]): x [rows, K] is quantised as above within the call, the sum is
- * exact.  w [N, K] int8 (row stride in bytes), w_scale [N] f32, bias [N] in x's type or NULL, y [rows, N] in x's type,
- * row stride in elements. */
+ * exact, its conversion to f32 (where it is above 2^24), the two scalings, the bias and the output's type round once each.
+ * w [N, K] int8 (row stride in bytes), w_scale [N] f32, bias [N] in x's type or NULL, y [rows, N] in x's type, row stride in elements. */
 int64_t vox_hip_linear_i8_workspace(int dtype, int64_t rows, int K, int N, const int8_t *w, int64_t w_stride);      /* (reads w's alignment) */
 int vox_hip_linear_i8(int dtype, const void *x, int64_t x_stride, int64_t rows, int K, int N, const int8_t *w, int64_t w_stride,
                       const float *w_scale, const void *bias, void *y, int64_t y_stride, void *ws, size_t ws_bytes, int device, void *stream);

@@ -1,6 +1,6 @@
 // vox_ops_call.cpp — the calls of voxtral_c_amd/ops.py on torch tensors, compiled: a short kernel's call is bound by the host, and most of that was the
-// interpreter (a call of a few tensors: attribute lookups, shape comparisons, argument conversions).  Measured, by ctypes / here: plan + accept + commit 31 / 17 us, scores
-// of one row 18.8 / 12.0, linear_i8 1 x 1280 x 6144 9.7 / 5.8, attention of 2 nodes 17 / 14 (now its kernels').  Bound by the launches, 3.2 us each.
+// interpreter (a call of a few tensors: attribute lookups, shape comparisons, argument conversions).  Measured, by ctypes / here: plan + accept + commit 31 / 16 us, scores
+// of one row 18.8 / 12.3, linear_i8 1 x 1280 x 6144 9.7 / 5.8, attention of 2 nodes 17 / 14.4 (now its kernels').  Bound by the launches, 3.2 us each.
 //
 // Each function takes the arguments of its namesake in ops.py, checks that they are what it takes without further ado, allocates results
 // and scratch memory from torch's allocator and calls the C entry (include/vox_hip_ops.h).  Anything else (a wrong shape, a table that is not contiguous, a tensor

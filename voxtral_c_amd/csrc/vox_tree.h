@@ -1,7 +1,7 @@
 // vox_tree.h — draft trees: ancestor sets, acceptance, and the accepted rows' way into the ring cache.
 // All three are bound by the latency of a launch and of one to three dependent trips to memory; a tree has at most 256 nodes, so one workgroup
 // with a thread per node holds all of it and every step is a constant number of barriers.  Measured, plan / accept / commit: one tree of 2
-// nodes, 26 layers of 8 x 128 f32: 1.5 / 2.5 / 3.8 us; 8 trees of 63 nodes in bf16: 3.7 / 3.9 / 4.0 us.  The three calls from Python take 17 us: the host
+// nodes, 26 layers of 8 x 128 f32: 1.4 / 2.4 / 3.4 us; 8 trees of 63 nodes in bf16: 3.4 / 3.5 / 3.6 us.  The three calls from Python take 15.6 us: the host
 // is the bound (three launches are 10 of them).
 #pragma once
 #include "vox_ops_common.h"

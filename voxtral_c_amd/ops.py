@@ -13,8 +13,9 @@ A verification pass takes several drafted tokens through the decoder at once::
 Every function enqueues HIP kernels on torch's current stream of the tensors' device and returns without waiting; results and scratch
 memory come from torch's allocator, so the calls may be captured into a graph.  Types: float32, bfloat16, float16 (one for all of a
 call's tensors), int32 for lengths, tokens and tree tables, int64 for the 64-bit words of ancestor sets.  Wrong arguments raise
-ValueError, a failed launch raises VoxError.  There are no derivatives: tensors that need gradients, or carry a
-forward-mode tangent, are refused.
+ValueError, what only the library finds wrong (a scale of 0, a batch beyond its grids) and a failed launch VoxError.  Sums and softmax statistics are
+float32; in the 16-bit types the attention's weights are rounded to the type in front of their product with the values.  There are no
+derivatives: tensors that need gradients, or carry a forward-mode tangent, are refused.
 """
 import ctypes as C
 import struct
