@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_ops import check_linear
+from test_gpu_ops import attn_case, check_linear
 
 import voxtral_c_amd as v
 from voxtral_c_amd import ops
@@ -195,3 +195,23 @@ def test_tree_attention_f32_numbers_whose_parts_are_all_as_large_as_can_be(T, G,
     want = (q[..., 1].double() * k[..., 1].double() * 0.75).cpu().numpy()
     # left out: 2^-21; the six products' sum: 6 e; the scale and its way to base 2 and back (two constants, three products): 5 e
     assert (np.abs(lse.cpu().double().numpy() / want - 1) <= 2.0 ** -21 + 11 * 2.0 ** -24).all()
+
+
+# ---- numbers of other kinds ----------------------------------------------------------------------------------------------------
+def test_whole_numbers_of_other_kinds_are_taken():
+    """numpy's integers and tensors of one whole number count as `top` and `window`; fractions are refused, not cut."""
+    rng = np.random.default_rng(5)
+    c = attn_case(5, F32, 1, 3, 4, 2, 64, 40, [33])
+    x = torch.as_tensor(rng.standard_normal((3, 50)).astype(np.float32)).to(DEV)
+    want, scores = ops.tree_attention(**c, window=9, scale=0.5), ops.token_scores(x, None, 3)
+    for whole in (np.int64, np.int32, torch.tensor):
+        assert torch.equal(ops.tree_attention(**c, window=whole(9), scale=np.float32(0.5)), want)
+        assert torch.equal(ops.token_scores(x, None, whole(3)).top_index, scores.top_index)
+    assert ops.token_scores(x, None, True).top_index.shape == (3, 1)
+    for wrong in (9.5, "9", None):
+        with pytest.raises(ValueError, match="window"):
+            ops.tree_attention(**c, window=wrong)
+        with pytest.raises(ValueError, match="top"):
+            ops.token_scores(x, None, wrong)
+    with pytest.raises(ValueError, match="scale"):
+        ops.tree_attention(**c, scale="1")

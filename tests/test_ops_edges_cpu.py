@@ -136,3 +136,13 @@ def test_tree_attention_takes_scales_whose_base_2_form_is_finite(scale, fine):
     args = ops._ATTN.pack(*[4096] * 10, *[8] * 18, 0, 1, 2, 4, 2, 64, 8, 0, scale, 0)
     assert (ops.hip.vox_hip_tree_attention_workspace(args) >= 0) == fine
     assert fine or "scale" in ops.hip.vox_hip_last_error().decode()
+
+
+def test_sizes_of_nothing_are_refused_by_name():
+    z, n, t, a = torch.zeros, torch.zeros(1, dtype=I32), torch.zeros(1, 2, dtype=I32), torch.zeros(1, 2, 1, dtype=torch.int64)
+    with pytest.raises(ValueError, match="tree_attention: 2 heads over 1 kv heads of 0"):
+        ops.tree_attention(z(1, 2, 2, 0), z(1, 2, 1, 0), z(1, 2, 1, 0), z(1, 5, 1, 0), z(1, 5, 1, 0), n, a, t)
+    with pytest.raises(ValueError, match="window 9.5: a whole number"):
+        ops.tree_attention(z(1, 2, 2, 4), z(1, 2, 1, 4), z(1, 2, 1, 4), z(1, 5, 1, 4), z(1, 5, 1, 4), n, a, t, window=9.5)
+    with pytest.raises(ValueError, match="top 1.5: a whole number"):
+        ops.token_scores(z(2, 3), None, 1.5)

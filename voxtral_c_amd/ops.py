@@ -18,6 +18,7 @@ float32; in the 16-bit types the attention's weights are rounded to the type in 
 derivatives: tensors that need gradients, or carry a forward-mode tangent, are refused.
 """
 import ctypes as C
+import operator
 import struct
 import warnings
 from collections import namedtuple
@@ -103,6 +104,14 @@ def _sizes(who, *tensors):
             raise ValueError(f"{who}: shape {tuple(t.shape)}: sizes of 2^31 and more are not supported")
 
 
+def _whole(who, name, number):
+    """A whole number of any kind (Python's, numpy's, a tensor of one) as Python's own."""
+    try:
+        return operator.index(number)
+    except TypeError:
+        raise ValueError(f"{who}: {name} {number!r}: a whole number is needed") from None
+
+
 def _device(who, *tensors):
     """The tensors' one GPU, as its number; all of a call's tensors are seen here, and what lies in their memory has to be their values."""
     d = tensors[0].get_device()
@@ -172,6 +181,11 @@ def tree_attention(q, k, v, k_cache, v_cache, cache_len, ancestors, depth, scale
     _nodes(who, q.shape)
     if Hk < 1 or H % Hk or not 1 <= D <= 256 or cap < 1:
         raise ValueError(f"{who}: {H} heads over {Hk} kv heads of {D} (at most 256), a cache of {cap} rows")
+    window = _whole(who, "window", window)
+    try:
+        scale = D ** -0.5 if scale is None else float(scale * 1.0)
+    except TypeError:
+        raise ValueError(f"{who}: scale {scale!r}: a number is needed") from None
     cache = (B, cap, Hk, D)
     number = _float_args(who, "q", q, q.shape, "k", k, (B, T, Hk, D), "v", v, (B, T, Hk, D), "k_cache", k_cache, cache, "v_cache", v_cache, cache)
     cache_len = _table(who, "cache_len", cache_len, (B,))
@@ -182,7 +196,7 @@ def tree_attention(q, k, v, k_cache, v_cache, cache_len, ancestors, depth, scale
     lse = q.new_empty((B, T, H), dtype=torch.float32) if return_lse else None
     args = _ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), cache_len.data_ptr(), ancestors.data_ptr(), depth.data_ptr(),
                       out.data_ptr(), 0 if lse is None else lse.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *k_cache.stride()[:3], *v_cache.stride()[:3],
-                      T * H * D, H * D, D, number, B, T, H, Hk, D, cap, max(-1, min(int(window), 0x7fffffff)), D ** -0.5 if scale is None else scale, 0)
+                      T * H * D, H * D, D, number, B, T, H, Hk, D, cap, max(-1, min(window, 0x7fffffff)), scale, 0)
     need = hip.vox_hip_tree_attention_workspace(args)
     ws = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
     if need < 0 or hip.vox_hip_tree_attention(args, None if ws is None else ws.data_ptr(), need, d, _stream(d)):
@@ -262,7 +276,7 @@ def token_scores(logits, tokens=None, top=0):
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"{who}: logits have the shape {tuple(logits.shape)}: [rows, vocab] is needed")
     R, V = logits.shape
-    number = _float_args(who, "logits", logits, logits.shape)
+    number, top = _float_args(who, "logits", logits, logits.shape), _whole(who, "top", top)
     if not 0 <= top <= min(MAX_TOP, V):
         raise ValueError(f"{who}: top {top} of {V} (at most {MAX_TOP})")
     shape = (R, 0)
